@@ -460,6 +460,92 @@ int tf_gemv_q6k_head_argmax(const uint8_t *w, const float *x,
 int tf_argmax_key_finalize(unsigned long long *amax_key, int *out_idx,
                            tf_stream_t stream);
 
+/* ------------------------------------ around the attention: 8-bit K/V cache
+ * No counterpart in the reference.  An 8-bit cache row is the Q8 of
+ * tf_quantize_q8: int8 k8[seq][n] and f32 kd[seq][n/32] (v8, vd alike), n =
+ * n_kv*head_dim, d = amax * fl(1/127), q = rint_even(x / d), value = q * d:
+ * 36 bytes per 32 values where f16 takes 64.  Values are finite. */
+
+#define TF_KV_F32 0 /* element types of the rows written and read back */
+#define TF_KV_F16 1
+
+/* RMS norm of every q and k head (weights q_norm / k_norm of head_dim values;
+ * NULL: none for it) and the NeoX rotation (i, i + head_dim/2) by pos *
+ * theta^(-2i/head_dim), in one pass, for n_tok tokens at positions pos0 + t
+ * (or *pos0_dev + t): y = x * (1 / sqrt(mean(x^2) + eps)) * w, then turned.
+ * The angle is formed in 64 bits (tf_rope_neox keeps the reference's f32
+ * angle).  Row t of q starts at q + t*q_stride (q, k and v may lie side by
+ * side in one projection's rows); q_out and k_out are tight rows and may be
+ * q and k themselves if those are tight.  head_dim even, <= 256. */
+int tf_qk_norm_rope(const float *q, int q_stride, const float *k, int k_stride,
+                    const float *q_norm, const float *k_norm, float eps,
+                    float *q_out, float *k_out, int n_head, int n_kv,
+                    int head_dim, int n_tok, int pos0, const int *pos0_dev,
+                    float theta, tf_stream_t stream);
+/* The same with k and v appended at cache rows pos0 + t: to the f16 cache
+ * (rounded as tf_copy_kv_f16), */
+int tf_qk_norm_rope_append(const float *q, int q_stride, const float *k,
+                           int k_stride, const float *v, int v_stride,
+                           const float *q_norm, const float *k_norm, float eps,
+                           float *q_out, uint16_t *k_cache, uint16_t *v_cache,
+                           int n_head, int n_kv, int head_dim, int n_tok,
+                           int pos0, const int *pos0_dev, float theta,
+                           tf_stream_t stream);
+/* or to the 8-bit cache; head_dim % 32 == 0. */
+int tf_qk_norm_rope_append_kv8(const float *q, int q_stride, const float *k,
+                               int k_stride, const float *v, int v_stride,
+                               const float *q_norm, const float *k_norm,
+                               float eps, float *q_out, int8_t *k8, float *kd,
+                               int8_t *v8, float *vd, int n_head, int n_kv,
+                               int head_dim, int n_tok, int pos0,
+                               const int *pos0_dev, float theta,
+                               tf_stream_t stream);
+/* Rows k, v of src_type (row t at t*src_stride elements) into 8-bit cache rows
+ * pos0 + t (or *pos0_dev + t), bit-identical to tf_quantize_q8.  n % 32 == 0. */
+int tf_kv8_write(const void *k, const void *v, int src_type, int src_stride,
+                 int8_t *k8, float *kd, int8_t *v8, float *vd, int n, int pos0,
+                 const int *pos0_dev, int n_tok, tf_stream_t stream);
+/* Cache rows row0 .. row0 + n_rows - 1 as tight rows of dst_type: the f32
+ * product q * d, for f16 rounded to nearest (what tf_attn_prefill takes). */
+int tf_kv8_read(const int8_t *k8, const float *kd, const int8_t *v8,
+                const float *vd, void *k, void *v, int dst_type, int n,
+                int row0, int n_rows, tf_stream_t stream);
+/* tf_flash_decode over the 8-bit cache: one token's attention at positions
+ * 0 .. pos0 (or *pos0_dev; a position of -1 has nothing to attend to and
+ * gives zeros), and with q8/d8 the Q8 of its output.  head_dim 64, 128 or
+ * 256, n_head/n_kv <= 16, 1 <= n_split <= 1024; partial holds n_head *
+ * n_split * (2 + head_dim) floats. */
+int tf_flash_decode_kv8(const float *q, const int8_t *k8, const float *kd,
+                        const int8_t *v8, const float *vd, float *partial,
+                        float *out, int8_t *q8, float *d8, int n_head, int n_kv,
+                        int head_dim, int pos0, const int *pos0_dev, int n_split,
+                        float scale, tf_stream_t stream);
+/* The split count this library recommends for it (1 .. 256). */
+int tf_flash_decode_kv8_n_split(int n_kv, int head_dim, int max_seq);
+
+/* ----------------------------------------------------------------- sampling */
+
+/* No counterpart in the reference.  One token a row from logits
+ * [n_rows][row_stride], n_vocab < 2^19 of them used: with z = logit /
+ * temperature and w = exp(z - max z) in 64 bits, in the order of falling
+ * logits (ties by rising index), top_k keeps the first k; top_p of these the
+ * shortest run whose sum reaches p of theirs; min_p of these those with w >=
+ * min_p.  out_idx = the first kept index in vocabulary order at which the
+ * running sum of kept w exceeds u times their sum.
+ * temperature, top_k, top_p, min_p: a value a row, or NULL (1, off, off, off);
+ * top_k <= 0 or >= n_vocab, top_p >= 1 and min_p <= 0 (and NaN) are off,
+ * top_p <= 0 keeps one token, min_p > 1 counts as 1; temperature <= 0 (or NaN)
+ * takes the largest logit, lowest index first.  u: a number in [0, 1) a row.
+ * NaN and -inf are never drawn, +inf before all else; a row with nothing to
+ * draw gives 0.  ws (16-byte aligned) holds tf_sample_ws_bytes(n_rows,
+ * n_vocab) bytes, which calls that run at the same time do not share. */
+int tf_sample(const float *logits, int n_rows, int n_vocab, int row_stride,
+              const float *temperature, const int *top_k, const float *top_p,
+              const float *min_p, const float *u, int *out_idx, void *ws,
+              long long ws_bytes, tf_stream_t stream);
+/* Bytes of its workspace; -1 for sizes that it does not take. */
+long long tf_sample_ws_bytes(int n_rows, int n_vocab);
+
 /* ----------------------------------------------------- decode-step runtime */
 /* C++ restatement of the reference model runtime for dense Qwen2-style
  * models (cuda/forward.rs:42-407, cuda/layer.rs:99-709,1210-1456,2125-2259,

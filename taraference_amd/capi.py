@@ -72,6 +72,16 @@ SIGNATURES: dict[str, list] = {
     "tf_rope_neox": [_P, _I, _I, _I, _P, _F, _P],
     "tf_copy_kv_f16": [_P, _P, _I, _P, _I, _P],
     "tf_argmax": [_P, _I, _P, _P],
+    "tf_qk_norm_rope": [_P, _I, _P, _I, _P, _P, _F, _P, _P, _I, _I, _I, _I, _I, _P, _F, _P],
+    "tf_qk_norm_rope_append": [_P, _I, _P, _I, _P, _I, _P, _P, _F, _P, _P, _P, _I, _I, _I, _I,
+                               _I, _P, _F, _P],
+    "tf_qk_norm_rope_append_kv8": [_P, _I, _P, _I, _P, _I, _P, _P, _F, _P, _P, _P, _P, _P, _I,
+                                   _I, _I, _I, _I, _P, _F, _P],
+    "tf_kv8_write": [_P, _P, _I, _I, _P, _P, _P, _P, _I, _I, _P, _I, _P],
+    "tf_kv8_read": [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P],
+    "tf_flash_decode_kv8": [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _I, _F, _P],
+    "tf_flash_decode_kv8_n_split": [_I, _I, _I],
+    "tf_sample": [_P, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, C.c_longlong, _P],
     "tf_q4k_block_dots": [_P, _P, _P, _P, _I, _I, _I, _P],
     "tf_decode_step_quantize_q8": [_P, _I, _I, _P, _P, _P],
     "tf_stream_read_probe": [_P, C.c_longlong, _P, _I, _I, _I, _P],
@@ -79,6 +89,10 @@ SIGNATURES: dict[str, list] = {
     "tf_version": [],
     "tf_exported_symbol_count": [],
 }
+
+
+# element types of the rows that the 8-bit cache is written from and read into
+KV_F32, KV_F16 = 0, 1
 
 
 class HipError(RuntimeError):
@@ -106,6 +120,8 @@ def load(path: Path | str | None = None) -> C.CDLL:
         fn.restype = C.c_int
     lib.tf_exported_symbol.argtypes = [C.c_int]
     lib.tf_exported_symbol.restype = C.c_char_p
+    lib.tf_sample_ws_bytes.argtypes = [C.c_int, C.c_int]
+    lib.tf_sample_ws_bytes.restype = C.c_longlong
     _lib = lib
     return lib
 
@@ -141,6 +157,7 @@ BOUND_ELSEWHERE = {"tf_model_create", "tf_model_destroy", "tf_model_forward",
                    "tf_model_logits", "tf_model_prefill", "tf_model_keep_stage_vectors",
                    "tf_model_stage_vector", "tf_model_q8_record",
                    "tf_model_k_cache", "tf_model_v_cache", "tf_exported_symbol",
+                   "tf_sample_ws_bytes",
                    # taraference_amd/gguf.py
                    "tf_gguf_open", "tf_gguf_close", "tf_gguf_version", "tf_gguf_data_offset",
                    "tf_gguf_file_size", "tf_gguf_n_tensors", "tf_gguf_tensor_at",

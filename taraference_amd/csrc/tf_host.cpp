@@ -131,6 +131,15 @@ static const char* const k_symbols[] = {
     "tf_rope_neox",
     "tf_copy_kv_f16",
     "tf_argmax",
+    "tf_qk_norm_rope",
+    "tf_qk_norm_rope_append",
+    "tf_qk_norm_rope_append_kv8",
+    "tf_kv8_write",
+    "tf_kv8_read",
+    "tf_flash_decode_kv8",
+    "tf_flash_decode_kv8_n_split",
+    "tf_sample",
+    "tf_sample_ws_bytes",
     "tf_gguf_open",
     "tf_gguf_close",
     "tf_gguf_version",

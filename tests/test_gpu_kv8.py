@@ -1,0 +1,195 @@
+"""The 8-bit K/V cache: rows written and read back, one token's attention over it."""
+import numpy as np
+import pytest
+import torch
+
+import _op_ref as ref
+import oracle
+from _gpu import KEEP, P, S, call, dev, empty, host
+
+pytestmark = pytest.mark.gpu
+
+
+def rows(rng, t, n):
+    x = rng.standard_normal((t, n)).astype(np.float32)
+    x *= np.float32(10.0) ** rng.integers(-6, 5, (t, n // 32)).astype(np.float32).repeat(32, 1)
+    x[:, :32] = 0  # a group without any value
+    if t > 1:
+        x[1, 32:64] = 1e-42 * np.arange(32)  # subnormal
+    return x
+
+
+@pytest.mark.parametrize("src", ["f32", "f16"])
+@pytest.mark.parametrize("n,t,pos,spare", [(128, 1, 0, 0), (256, 1, 17, 0), (512, 300, 1000, 64),
+                                           (64, 5, 3, 5), (1024, 33, 0, 0), (2048, 7, 9, 32),
+                                           (32, 70001, 2, 0), (96, 11, 1, 1)])
+def test_write_and_read(gpu, n, t, pos, spare, src):
+    rng = np.random.default_rng(n + t)
+    # f16 rows lie in f16's range
+    k, v = (rows(rng, t, n + 32)[:, :n] if src == "f32" else
+            rng.standard_normal((t, n)).astype(np.float16).astype(np.float32) for _ in range(2))
+    stride = n + spare
+    ty = np.float32 if src == "f32" else np.float16
+    dk, dv = (dev(np.concatenate([a.astype(ty), np.full((t, spare), 9e9 if src == "f32" else 6e4,
+                                                        ty)], 1)) for a in (k, v))
+    k8, v8 = (dev(np.full((pos + t + 1, n), 77, np.int8)) for _ in range(2))
+    kd, vd = (dev(np.full((pos + t + 1, n // 32), -3, np.float32)) for _ in range(2))
+    call("tf_kv8_write", P(dk), P(dv), gpu.KV_F32 if src == "f32" else gpu.KV_F16, stride, P(k8),
+         P(kd), P(v8), P(vd), n, pos, None, t, S())
+    for x, c8, cd in ((k, k8, kd), (v, v8, vd)):
+        q, d = oracle.quantize_q8(np.ascontiguousarray(x).reshape(-1))
+        g8, gd = host(c8), host(cd)
+        assert np.array_equal(g8[pos:pos + t].ravel(), q)
+        assert np.array_equal(gd[pos:pos + t].ravel(), d)
+        assert (g8[:pos] == 77).all() and (g8[pos + t:] == 77).all()
+        assert (gd[:pos] == -3).all() and (gd[pos + t:] == -3).all()
+        f32 = (g8[pos:pos + t].reshape(-1, 32).astype(np.float32) *
+               gd[pos:pos + t].reshape(-1, 1)).reshape(t, n)
+        for dst in ("f32", "f16"):
+            ty = torch.float32 if dst == "f32" else torch.float16
+            a, b = empty((t + 1, n), ty).fill_(5), empty((t + 1, n), ty).fill_(5)
+            call("tf_kv8_read", P(k8), P(kd), P(v8), P(vd), P(a), P(b),
+                 gpu.KV_F32 if dst == "f32" else gpu.KV_F16, n, pos, t, S())
+            got = host(a if c8 is k8 else b)
+            with np.errstate(over="ignore"):
+                assert np.array_equal(got[:t], f32.astype(got.dtype))
+            assert (got[t] == 5).all()
+
+
+def test_write_at_a_device_position(gpu):
+    n, t = 128, 3
+    x = np.random.default_rng(3).standard_normal((t, n)).astype(np.float32)
+    d, pos = dev(x), dev(np.array([4], np.int32))
+    k8, v8 = (dev(np.zeros((9, n), np.int8)) for _ in range(2))
+    kd, vd = (dev(np.zeros((9, n // 32), np.float32)) for _ in range(2))
+    call("tf_kv8_write", P(d), P(d), gpu.KV_F32, n, P(k8), P(kd), P(v8), P(vd), n, 0, P(pos), t, S())
+    q, s = ref.q8_rows(x)
+    for c8, cd in ((k8, kd), (v8, vd)):
+        assert np.array_equal(host(c8)[4:7], q) and np.array_equal(host(cd)[4:7], s)
+        assert not host(c8)[:4].any() and not host(c8)[7:].any()
+
+
+def cache(rng, seq, n, spread=1.0):
+    x = (spread * rng.standard_normal((seq, n))).astype(np.float32)
+    x[:, ::17] *= 5  # a few channels larger than the rest
+    return ref.q8_rows(x)
+
+
+def attend(q, k8, kd, v8, vd, n_kv, pos, n_split, scale, pos_dev=None, want_q8=False):
+    h, hd = q.shape
+    part, out = empty(h * n_split * (2 + hd)).fill_(float("nan")), empty(h * hd)
+    q8, d8 = (empty(h * hd, torch.int8), empty(h * hd // 32)) if want_q8 else (None, None)
+    call("tf_flash_decode_kv8", P(dev(q)), P(k8), P(kd), P(v8), P(vd), P(part), P(out), P(q8),
+         P(d8), h, n_kv, hd, pos, P(pos_dev), n_split, scale, S())
+    return (host(out).reshape(h, hd),) + ((host(q8), host(d8)) if want_q8 else ())
+
+
+def check(got, q, k, v, n_kv, scale):
+    want, tol = ref.attention(q, k, v, n_kv, scale)
+    err = np.abs(got - want)
+    assert (err <= tol).all(), (err / np.maximum(tol, 1e-300)).max()
+
+
+GROUPS = [(16, 2, 128), (28, 4, 128), (14, 2, 64), (16, 4, 256), (5, 5, 64), (16, 1, 128),
+          (3, 1, 256), (16, 1, 64), (15, 1, 256), (8, 8, 128)]
+
+
+@pytest.mark.parametrize("h,kv,hd", GROUPS)
+@pytest.mark.parametrize("seq,n_split", [(1, 1), (1, 8), (2, 1), (31, 1), (33, 2), (130, 8), (257, 1),
+                                         (1000, 3), (1025, 16), (4099, 64)])
+def test_attention(gpu, h, kv, hd, seq, n_split):
+    rng = np.random.default_rng(seq + hd)
+    q = rng.standard_normal((h, hd)).astype(np.float32)
+    k8, kd = cache(rng, seq, kv * hd)
+    v8, vd = cache(rng, seq, kv * hd)
+    scale = 1 / np.sqrt(hd)
+    # rows behind the position hold what must not be read into anything
+    def behind(a, fill):
+        return dev(np.concatenate([a, np.full((40, a.shape[1]), fill, a.dtype)]))
+    got = attend(q, behind(k8, 127), behind(kd, np.nan), behind(v8, -127), behind(vd, np.inf), kv,
+                 seq - 1, n_split, scale)[0]
+    check(got, q, ref.q8_values(k8, kd), ref.q8_values(v8, vd), kv, scale)
+
+
+@pytest.mark.parametrize("h,kv,hd", [(16, 2, 128), (14, 2, 64), (6, 2, 256)])
+@pytest.mark.parametrize("case", ["sink", "tiny", "huge", "flat", "zero_q", "mixed_scales"])
+def test_attention_values(gpu, h, kv, hd, case):
+    rng = np.random.default_rng(hd)
+    seq, n = 700, kv * hd
+    q = rng.standard_normal((h, hd)).astype(np.float32)
+    k = rng.standard_normal((seq, n)).astype(np.float32)
+    v = rng.standard_normal((seq, n)).astype(np.float32)
+    scale = 1 / np.sqrt(hd)
+    if case == "sink":  # one key far above the rest, late and early
+        k[[0, 650]] *= 12
+    elif case == "tiny":
+        v *= 1e-20
+        k *= 1e-12
+    elif case == "huge":
+        v *= 1e25
+        k *= 1e9
+        scale = scale * 1e-9
+    elif case == "flat":
+        k[:] = 0
+    elif case == "zero_q":
+        q[:] = 0
+    else:  # scales of neighbouring groups and rows 10^12 apart
+        v *= (10.0 ** rng.integers(-6, 7, (seq, n // 32))).repeat(32, 1).astype(np.float32)
+        v[::3] = 0
+    k8, kd = ref.q8_rows(k)
+    v8, vd = ref.q8_rows(v)
+    got = attend(q, dev(k8), dev(kd), dev(v8), dev(vd), kv, seq - 1, 4, scale)[0]
+    check(got, q, ref.q8_values(k8, kd), ref.q8_values(v8, vd), kv, scale)
+
+
+def test_attention_q8_device_position_and_empty(gpu):
+    h, kv, hd, seq = 28, 4, 128, 600
+    rng = np.random.default_rng(5)
+    q = rng.standard_normal((h, hd)).astype(np.float32)
+    k8, kd = cache(rng, seq, kv * hd)
+    v8, vd = cache(rng, seq, kv * hd)
+    c = [dev(a) for a in (k8, kd, v8, vd)]
+    scale = 1 / np.sqrt(hd)
+    k, v = ref.q8_values(k8, kd), ref.q8_values(v8, vd)
+    pos = torch.zeros(1, dtype=torch.int32, device="cuda")
+    KEEP.append(pos)
+    for n_split in (1, 8):
+        for at in (599, 0, 64, -1):
+            pos.fill_(at)
+            out, q8, d8 = attend(q, *c, kv, 0, n_split, scale, pos_dev=pos, want_q8=True)
+            check(out, q, k[:at + 1], v[:at + 1], kv, scale)
+            wq, wd = oracle.quantize_q8(out.reshape(-1))
+            assert np.array_equal(q8, wq) and np.array_equal(d8, wd)
+
+
+def test_attention_long(gpu):
+    """A cache whose element offsets pass 2^31: only its last rows and first rows
+    hold anything, and the query finds them."""
+    h, kv, hd = 8, 8, 256
+    seq, n = 1_100_000, 8 * 256
+    k8 = torch.zeros(seq, n, dtype=torch.int8, device="cuda")
+    v8 = torch.zeros(seq, n, dtype=torch.int8, device="cuda")
+    kd = torch.ones(seq, n // 32, device="cuda")
+    vd = torch.ones(seq, n // 32, device="cuda")
+    KEEP.extend([k8, v8, kd, vd])
+    rng = np.random.default_rng(2)
+    q = rng.standard_normal((h, hd)).astype(np.float32)
+    scale = 1 / np.sqrt(hd)
+    for r in (3, seq - 2):
+        k8[r] = torch.from_numpy(np.clip(np.rint(q.reshape(-1) * 20), -127, 127).astype(np.int8))
+        v8[r] = (r % 100) + 1
+    n_split = gpu.load().tf_flash_decode_kv8_n_split(kv, hd, seq)
+    got = attend(q, k8, kd, v8, vd, kv, seq - 1, n_split, scale)[0]
+    kk = np.clip(np.rint(q * 20), -127, 127)
+    x = (kk * q).sum(1) * scale  # both rows' score; the others score 0
+    e = np.exp(-x)
+    want = ((3 % 100 + 1) + ((seq - 2) % 100 + 1)) / (2 + (seq - 2) * e)
+    assert np.abs(got - want[:, None]).max() <= 2e-4 * want.max()
+
+
+def test_split_counts(gpu):
+    f = gpu.load().tf_flash_decode_kv8_n_split
+    for kv in (1, 2, 4, 8, 32, 300):
+        for hd in (64, 128, 256):
+            for seq in (1, 100, 5000, 131072, 10**7):
+                assert 1 <= f(kv, hd, seq) <= 256

@@ -1,0 +1,146 @@
+"""Sampling against the 64-bit definition: the same token, exactly."""
+import numpy as np
+import pytest
+import torch
+
+import _op_ref as ref
+from _gpu import KEEP, P, S, call, dev, empty, host
+
+pytestmark = pytest.mark.gpu
+
+
+def draw(gpu, x, u, t=None, k=None, p=None, m=None, stride=None):
+    r, n = x.shape
+    if stride:
+        x = np.concatenate([x, np.full((r, stride - n), 99, np.float32)], 1)
+    d = [None if a is None else dev(np.asarray(a, ty))
+         for a, ty in ((t, np.float32), (k, np.int32), (p, np.float32), (m, np.float32))]
+    out, size = empty(r, torch.int32), gpu.load().tf_sample_ws_bytes(r, n)
+    ws = empty(size, torch.uint8).fill_(0xA5)
+    call("tf_sample", P(dev(x)), r, n, stride or n, *(P(a) for a in d),
+         P(dev(np.asarray(u, np.float32))), P(out), P(ws), size, S())
+    return host(out)
+
+
+def want(x, u, t=None, k=None, p=None, m=None):
+    r = x.shape[0]
+    pick = lambda a, i, off: off if a is None else np.asarray(a)[i]  # noqa: E731
+    return np.array([ref.sample(x[i], pick(t, i, 1.0), pick(k, i, 0), np.float32(pick(p, i, 1.0)),
+                                np.float32(pick(m, i, 0.0)), u[i]) for i in range(r)])
+
+
+def logits(rng, r, n, body=2.2):
+    x = (body * rng.standard_normal((r, n))).astype(np.float32)
+    for i in range(r):
+        at = rng.integers(0, n, min(n, 30))
+        x[i, at] += rng.uniform(2, 12, at.size).astype(np.float32)
+    return x
+
+
+SIZES = [(1, 1), (1, 2), (3, 7), (2, 63), (5, 64), (2, 65), (1, 1000), (3, 4097), (2, 8192),
+         (2, 8193), (1, 32000), (2, 50257), (1, 151936), (2, 262145), (1, 524287)]
+
+
+@pytest.mark.parametrize("r,n", SIZES)
+@pytest.mark.parametrize("filters", ["none", "k", "p", "m", "all"])
+def test_random(gpu, r, n, filters):
+    rng = np.random.default_rng(r * n)
+    for trial in range(3):
+        x, u = logits(rng, r, n), rng.random(r).astype(np.float32)
+        a = {"t": rng.uniform(0.3, 2.0, r).astype(np.float32)}
+        if filters in ("k", "all"):
+            a["k"] = rng.choice([0, 1, 2, 40, 1000, n, n + 5], r)
+        if filters in ("p", "all"):
+            a["p"] = rng.choice([0.0, 0.1, 0.5, 0.9, 0.99, 1.0, 2.0], r)
+        if filters in ("m", "all"):
+            a["m"] = rng.choice([0.0, 0.001, 0.05, 0.3, 1.0, 7.0], r)
+        got = draw(gpu, x, u, **a, stride=n + 3 if trial == 1 else None)
+        assert np.array_equal(got, want(x, u, **a)), a
+
+
+@pytest.mark.parametrize("n", [257, 20001, 151936])
+def test_flat_and_hot(gpu, n):
+    """Distributions whose cut lies among tens of thousands of near-equal tokens."""
+    rng = np.random.default_rng(n)
+    x = (0.01 * rng.standard_normal((6, n))).astype(np.float32)
+    u = rng.random(6).astype(np.float32)
+    for t in (1.0, 50.0, 1e-3):
+        for p in (0.3, 0.95):
+            a = dict(t=[t] * 6, p=[p] * 6, k=[0, 0, n // 2, n // 3, 17, 0], m=[0, 0.99, 0, 0, 0, 0.5])
+            assert np.array_equal(draw(gpu, x, u, **a), want(x, u, **a)), (t, p)
+
+
+@pytest.mark.parametrize("n", [5, 1030, 151936])
+def test_ties(gpu, n):
+    """Equal logits: the lowest indices are kept, -0 equals +0."""
+    rng = np.random.default_rng(n)
+    x = np.zeros((8, n), np.float32)
+    x[1] = -3.5
+    x[2, ::2] = -0.0
+    x[3] = rng.integers(0, 2, n)
+    x[4] = rng.integers(0, 5, n)
+    x[5] = np.finfo(np.float32).min
+    x[6] = np.finfo(np.float32).max
+    x[7, n // 2] = 40.0
+    u = np.array([0, 0.25, 0.5, 0.9, 0.75, 1 - 2.0**-24, 0.3, 0.999], np.float32)
+    for a in ({}, {"k": [3] * 8}, {"p": [0.5] * 8}, {"k": [max(1, n // 2)] * 8, "p": [0.75] * 8},
+              {"m": [0.5] * 8}, {"k": [n - 1] * 8, "m": [1.0] * 8, "p": [0.25] * 8}):
+        assert np.array_equal(draw(gpu, x, u, **a), want(x, u, **a)), a
+
+
+def test_masked_and_infinite(gpu):
+    n = 9001
+    rng = np.random.default_rng(4)
+    x = logits(rng, 10, n)
+    x[0] = -np.inf                     # nothing to draw
+    x[1] = np.nan
+    x[2, rng.random(n) < 0.9] = -np.inf
+    x[3, rng.random(n) < 0.9] = np.nan
+    x[4] = -np.inf
+    x[4, 8000] = -1e38                 # one token left
+    x[5, [7, 70, 700]] = np.inf        # shared by three
+    x[6, rng.random(n) < 0.99] = np.finfo(np.float32).min
+    x[7] = np.nan
+    x[7, 3:6] = -np.inf
+    x[8, :] = -np.inf
+    x[8, [100, 200]] = np.inf
+    x[9, ::2] = np.nan
+    for u in (0.0, 0.4, 0.99):
+        us = np.full(10, u, np.float32)
+        for a in ({}, {"k": [2] * 10}, {"k": [8000] * 10}, {"p": [0.9] * 10}, {"m": [0.1] * 10},
+                  {"t": [0.5] * 10, "k": [5000] * 10, "p": [0.99] * 10, "m": [0.01] * 10}):
+            assert np.array_equal(draw(gpu, x, us, **a), want(x, us, **a)), (u, a)
+
+
+def test_greedy_and_odd_settings(gpu):
+    rng = np.random.default_rng(6)
+    x = logits(rng, 6, 3001)
+    x[0, [10, 20]] = 50
+    u = np.full(6, 0.7, np.float32)
+    t = np.array([0, -1, np.nan, 1e-30, np.inf, 1], np.float32)
+    assert np.array_equal(draw(gpu, x, u, t=t), want(x, u, t=t))
+    assert draw(gpu, x, u, t=t)[0] == 10
+    nan = np.full(6, np.nan, np.float32)
+    off = draw(gpu, x, u)
+    assert np.array_equal(draw(gpu, x, u, p=nan, m=nan, k=[-4] * 6), off)
+    assert np.array_equal(off, want(x, u))
+    assert np.array_equal(draw(gpu, x, np.array([np.nan, -1, 1, 2, 0, 1], np.float32), k=[9] * 6),
+                          want(x, np.array([0, 0, 1, 2, 0, 1], np.float32), k=[9] * 6))
+
+
+def test_many_rows(gpu):
+    rng = np.random.default_rng(8)
+    x, u = logits(rng, 700, 1500), rng.random(700).astype(np.float32)
+    a = dict(t=rng.uniform(0.5, 1.5, 700).astype(np.float32), k=rng.integers(0, 100, 700),
+             p=rng.uniform(0.5, 1.05, 700).astype(np.float32),
+             m=rng.uniform(-0.05, 0.1, 700).astype(np.float32))
+    assert np.array_equal(draw(gpu, x, u, **a), want(x, u, **a))
+
+
+def test_a_distribution(gpu):
+    """Many draws of one row: each token as often as its weight says."""
+    w = np.array([0.5, 0.25, 0.125, 0.0625, 0.0625])
+    n = 4096
+    u = ((np.arange(n) + 0.5) / n).astype(np.float32)
+    got = draw(gpu, np.tile(np.log(w).astype(np.float32), (n, 1)), u)
+    assert np.array_equal(np.bincount(got, minlength=5), (w * n).astype(int))
