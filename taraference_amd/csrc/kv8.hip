@@ -5,6 +5,9 @@
 // values, d = amax * fl(1/127), q = rint_even(x / d); value = q * d.  36 bytes
 // per 32 values where f16 takes 64.  The scale is f32, as in that format, so
 // that rows of any magnitude keep their 7 bits.
+#include <math.h>
+
+#include "lds_dma.hpp"
 #include "tf_common.hpp"
 #include "tf_host.hpp"
 
@@ -60,62 +63,395 @@ __global__ __launch_bounds__(256) void tf_kv8_read_kernel(const int8_t* __restri
     else out[i] = __builtin_bit_cast(uint16_t, (_Float16)x);
 }
 
-// One head a wave, the split walked in tiles of 64 tokens.
+// ------------------------------------------- one token's attention
+//
+// out_h = sum_t softmax_t(scale q_h . K_t) V_t with K_t = kd[t][g] k8[t], V_t =
+// vd[t][g] v8[t] (g: 32 dims).  Grid (kv head, split); a workgroup reads each
+// byte of its split once, for the G query heads of the kv head.
+//
+// A wave owns the 32-token tiles j = wave, wave + W, ... of the split and moves
+// them HBM -> LDS itself (global_load_lds, no register staging) into a two-slot
+// ring of its own, one tile ahead; the waves meet only to share the query and
+// to merge their (m, l, O).  Per tile, on v_mfma_f32_16x16x32_f16 (lane l, n = l
+// % 16, g = l / 16: A[n][8g ..], B[8g ..][n], C[4g + r][n]):
+//   K Q^T  one k step is one scale group: A = 8 bytes of token n (or 16 + n), as
+//          f16 (exact), B = 8 dims of head n in two f16 parts after a power of
+//          two (2^-22 of the largest); the sums of a group are f32 and take the
+//          token's scale there.
+//   softmax of head n over the lane's tokens 4g + r and 16 + 4g + r, in f32.
+//          The maximum and the exponent below are renewed, and O rescaled, only
+//          where a lane found a larger one.
+//   V^T P^T with the tokens in the order in which the lane has them: A = 8 tokens
+//          of dim n (ds_read_b64_tr_b8), as f16 (exact); B = p vd[t][g] 2^f, for
+//          each group of dims, in two f16 parts.  f takes the largest scale met
+//          so far to [2^14, 2^15), so the parts end at 2^-39 of the largest
+//          product.
+// LDS rows keep their 16-byte chunks xor-ed with the row (the copies' sources
+// are permuted), so that the 16 rows that half a wave reads lie in distinct banks.
+typedef _Float16 tf_h2x __attribute__((ext_vector_type(2)));
+
 template <int HD>
-__global__ __launch_bounds__(256) void tf_flash_kv8_kernel(
+struct TfKv8 {
+    static constexpr int T = 32;                       // tokens per tile
+    static constexpr int W = HD == 256 ? 4 : 8;        // waves
+    static constexpr int NG = HD / 32, DB = HD / 16;
+    static constexpr int NC = HD / 16;                 // 16-byte chunks of a row
+    static constexpr int TILE = T * HD;                // bytes of K (or V)
+    static constexpr int SC = T * NG * 4;              // bytes of its scales
+    static constexpr int KOFF = 0, KDOFF = TILE, VDOFF = TILE + SC, VOFF = TILE + 2 * SC;
+    static constexpr int SLOT = 2 * (TILE + SC);
+    static constexpr int COPIES = TILE / 1024;         // 16 bytes a lane
+    static constexpr int K_COPIES = COPIES + (HD == 128 ? 1 : 2);  // K and both scales
+    static constexpr int PER = K_COPIES + COPIES;
+    static constexpr int LDS = W * 2 * SLOT;
+    static constexpr int CR = HD + 4;                  // merge row: m, l, pad, O
+    static_assert(16 * HD * 4 <= SLOT, "the query fits a slot");
+    static_assert(W * 16 * CR * 4 <= LDS, "the merge rows fit the ring");
+    // the chunk permutation of a K row (16 consecutive rows are read together) and
+    // of a V row (8a .. 8a + 7 and 16 + 8a .. are)
+    static __device__ __forceinline__ int kswz(int r) {
+        return HD == 64 ? (r >> 2) & 3 : HD == 128 ? (r >> 1) & 7 : r & 15;
+    }
+    static __device__ __forceinline__ int vswz(int r) {
+        return HD == 64    ? ((r >> 2) & 1) | ((r >> 4) << 1)
+               : HD == 128 ? ((r >> 1) & 3) | ((r >> 4) << 2)
+                           : (r & 7) | ((r >> 4) << 3);
+    }
+};
+
+// Eight int8 values as f16: with the sign bit flipped a byte is q + 128, behind
+// 0x64 the f16 number 1024 + q + 128, less 1152 exactly q.
+__device__ __forceinline__ tf_h16x8 tf_i8_f16(tf_u32x2 b) {
+    union {
+        uint32_t u[4];
+        tf_h2x h[4];
+        tf_h16x8 v;
+    } r;
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const uint32_t x = b[i] ^ 0x80808080u;
+        r.u[2 * i] = __builtin_amdgcn_perm(0x64646464u, x, 0x04010400u);
+        r.u[2 * i + 1] = __builtin_amdgcn_perm(0x64646464u, x, 0x04030402u);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) r.h[i] -= tf_h2x{(_Float16)1152.f, (_Float16)1152.f};
+    return r.v;
+}
+
+// a, b = hi + lo in f16 parts.  hi is opaque to the compiler, which would otherwise
+// round the product behind a value a second time, and not always alike, for lo's
+// difference (2^-11 of a value in one of 2^13: 4e-6 of an output of 5000 tokens).
+__device__ __forceinline__ void tf_kv8_split(float a, float b, tf_h2x& hi, tf_h2x& lo) {
+    uint32_t h = __builtin_bit_cast(uint32_t, tf_h2x{(_Float16)a, (_Float16)b});
+    asm("" : "+v"(h));
+    hi = __builtin_bit_cast(tf_h2x, h);
+    lo = tf_h2x{(_Float16)(a - (float)hi.x), (_Float16)(b - (float)hi.y)};
+}
+
+template <int N>
+__device__ __forceinline__ void tf_kv8_wait() {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+// With out (n_split == 1 only) the workgroup writes the output itself, and its
+// Q8 with q8, as tf_flash_decode does.
+template <int HD>
+__global__ __launch_bounds__(64 * TfKv8<HD>::W) void tf_flash_kv8_kernel(
     const float* __restrict__ q, const int8_t* __restrict__ k8, const float* __restrict__ kd,
     const int8_t* __restrict__ v8, const float* __restrict__ vd, float* __restrict__ partial,
-    int n_head, int n_kv, int pos0, const int* __restrict__ pos0_dev, int n_split, float scale) {
-    constexpr int DPL = HD / 64;
-    __shared__ float p_lds[4][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int h = blockIdx.x * 4 + wave, s = blockIdx.y;
-    if (h >= n_head) return;
-    const int kv_h = h / (n_head / n_kv);
+    int n_head, int n_kv, int pos0, const int* __restrict__ pos0_dev, int n_split, float scale,
+    float* __restrict__ out, int8_t* __restrict__ q8, float* __restrict__ d8) {
+    using L = TfKv8<HD>;
+    constexpr int NG = L::NG, DB = L::DB, W = L::W;
+    extern __shared__ __align__(16) uint8_t lds[];
+    const int kv_h = blockIdx.x, s = blockIdx.y, G = n_head / n_kv;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n = lane & 15, g = lane >> 4;
     if (pos0_dev) pos0 = pos0_dev[0];
     const int seq = pos0 + 1;
-    const int chunk = (seq + n_split - 1) / n_split;
+    // whole tiles a split
+    const int chunk = (int)((((long long)seq + n_split - 1) / n_split + L::T - 1) / L::T * L::T);
     const int t_begin = (int)min((long long)s * chunk, (long long)seq);
-    const int t_end = min(t_begin + chunk, seq);
-    const float* qh = q + (size_t)h * HD;
-    float m = TF_NEG_BIG, l = 0.f, o[DPL];
-    for (int i = 0; i < DPL; i++) o[i] = 0.f;
-    for (int t0 = t_begin; t0 < t_end; t0 += 64) {
-        const int t = t0 + lane;
-        float sc = TF_NEG_BIG;
-        if (t < t_end) {
-            const size_t row = ((size_t)t * n_kv + kv_h) * HD;
-            float acc = 0.f;
-            for (int g = 0; g < HD / 32; g++) {
-                float a = 0.f;
-                for (int i = 0; i < 32; i++) a = fmaf(qh[32 * g + i], (float)k8[row + 32 * g + i], a);
-                acc = fmaf(a, kd[row / 32 + g], acc);
-            }
-            sc = acc * scale;
+    const int t_end = (int)min((long long)t_begin + chunk, (long long)seq);
+    const int n_tiles = (t_end - t_begin + L::T - 1) / L::T;
+    const size_t row8 = (size_t)n_kv * HD, rowd = (size_t)n_kv * NG * 4;
+    uint8_t* ring = lds + wave * 2 * L::SLOT;
+
+    // the query's rows (heads past G repeat the last) into wave 0's second slot
+    constexpr int HPC = 1024 / (HD * 4);  // heads of a copy
+    const float* qk = q + (size_t)kv_h * G * HD;
+#pragma unroll
+    for (int i = 0; i < 16 / HPC; i++)
+        if (i % W == wave) {
+            const int h = min(i * HPC + lane / (HD / 4), G - 1);
+            tf_lds_dma16(qk + (size_t)h * HD + 4 * (lane % (HD / 4)),
+                         tf_lds_off(lds) + L::SLOT + 1024 * i);
         }
-        const float m_new = fmaxf(m, tf_wave_max(sc));
-        const float alpha = __expf(m - m_new);
-        const float e = t < t_end ? __expf(sc - m_new) : 0.f;
-        p_lds[wave][lane] = e;
-        l = l * alpha + tf_group_sum<64>(e);
-        m = m_new;
-        for (int i = 0; i < DPL; i++) o[i] *= alpha;
-        __builtin_amdgcn_wave_barrier();
-        for (int tt = 0; tt < min(64, t_end - t0); tt++) {
-            const size_t row = ((size_t)(t0 + tt) * n_kv + kv_h) * HD;
-            for (int i = 0; i < DPL; i++) {
-                const int dim = lane + 64 * i;
-                o[i] = fmaf(p_lds[wave][tt] * vd[(row + dim) / 32], (float)v8[row + dim], o[i]);
+    // tile j -> slot: K, the scales of K and V, V; rows past the split repeat its
+    // last (their weights are zero)
+    auto issue = [&](int j, int slot) {
+        const int t0 = t_begin + L::T * j, last = t_end - 1 - t0;
+        const uint32_t base = tf_lds_off(ring) + slot * L::SLOT;
+        const uint8_t* kb = reinterpret_cast<const uint8_t*>(k8) + (size_t)t0 * row8 + kv_h * HD;
+        const uint8_t* vb = reinterpret_cast<const uint8_t*>(v8) + (size_t)t0 * row8 + kv_h * HD;
+        const uint8_t* kdb = reinterpret_cast<const uint8_t*>(kd) + (size_t)t0 * rowd + kv_h * NG * 4;
+        const uint8_t* vdb = reinterpret_cast<const uint8_t*>(vd) + (size_t)t0 * rowd + kv_h * NG * 4;
+        constexpr int RPC = 64 / L::NC;  // rows of a copy
+#pragma unroll
+        for (int i = 0; i < L::COPIES; i++) {
+            const int r = RPC * i + lane / L::NC, c = (lane % L::NC) ^ L::kswz(r);
+            tf_lds_dma16(kb + (size_t)min(r, last) * row8 + 16 * c, base + L::KOFF + 1024 * i);
+        }
+        if constexpr (HD == 128) {
+            const int r = min(lane & 31, last);
+            tf_lds_dma16((lane < 32 ? kdb : vdb) + (size_t)r * rowd, base + L::KDOFF);
+        } else if constexpr (HD == 256) {
+            const size_t o = (size_t)min(lane >> 1, last) * rowd + 16 * (lane & 1);
+            tf_lds_dma16(kdb + o, base + L::KDOFF);
+            tf_lds_dma16(vdb + o, base + L::VDOFF);
+        } else {
+            const uint32_t o = (uint32_t)(min(lane >> 1, last) * (int)rowd + 4 * (lane & 1));
+            tf_lds_dma_s<4>(kdb, o, base + L::KDOFF);
+            tf_lds_dma_s<4>(vdb, o, base + L::VDOFF);
+        }
+#pragma unroll
+        for (int i = 0; i < L::COPIES; i++) {
+            const int r = RPC * i + lane / L::NC, c = (lane % L::NC) ^ L::vswz(r);
+            tf_lds_dma16(vb + (size_t)min(r, last) * row8 + 16 * c, base + L::VOFF + 1024 * i);
+        }
+    };
+    const bool any = wave < n_tiles;
+    if (any) {
+        issue(wave, 0);
+        tf_kv8_wait<L::PER>();  // the query's copies are older
+    } else {
+        tf_kv8_wait<0>();
+    }
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+
+    // the query of head n: dims 32 j + 8 g .. + 7 as two f16 parts of q 2^-e, the
+    // largest of the group's heads in [2^14, 2^15)
+    tf_h16x8 qa[NG][2];
+    {
+        const float* ql = reinterpret_cast<const float*>(lds + L::SLOT) + n * HD + 8 * g;
+        float qv[NG][8], qmax = 0.f;
+#pragma unroll
+        for (int j = 0; j < NG; j++)
+#pragma unroll
+            for (int i = 0; i < 8; i += 4) {
+                const float4 v = *reinterpret_cast<const float4*>(ql + 32 * j + i);
+                const float f = n < G ? 1.f : 0.f;
+                qv[j][i] = v.x * f, qv[j][i + 1] = v.y * f;
+                qv[j][i + 2] = v.z * f, qv[j][i + 3] = v.w * f;
+            }
+#pragma unroll
+        for (int j = 0; j < NG; j++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) qmax = fmaxf(qmax, fabsf(qv[j][i]));
+        qmax = tf_wave_max(qmax);
+        const int e = qmax > 0.f ? ilogbf(qmax) - 14 : 0;
+#pragma unroll
+        for (int j = 0; j < NG; j++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const float x = ldexpf(qv[j][i], -e);
+                const _Float16 h0 = (_Float16)x;
+                qa[j][0][i] = h0;
+                qa[j][1][i] = (_Float16)(x - (float)h0);
+            }
+        scale = ldexpf(scale, e);
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();  // the query has been read: its slot is free
+    asm volatile("" ::: "memory");
+    if (wave + W < n_tiles) issue(wave + W, 1);
+
+    float m = TF_NEG_BIG, l = 0.f;  // head n: the maximum, this lane's share of the sum
+    float vtop = 0.f, vf = 1.f;     // scales below vtop fit under the factor vf
+    tf_f32x4v o[DB];                // O^T of dims 16 b + 4 g + r, head n, times vf
+#pragma unroll
+    for (int b = 0; b < DB; b++) o[b] = tf_f32x4v{0.f, 0.f, 0.f, 0.f};
+    const int tr = ((lane & 15) >> 1);                             // the lane's row of a transposing read
+    const int vrow = (tr < 4 ? tr : 12 + tr) + 4 * g;              // its token
+    const uint32_t vbase = L::VOFF + vrow * HD + 8 * (lane & 1);
+    const int vx = L::vswz(vrow);
+
+    int slot = 0;
+    for (int j = wave; j < n_tiles; j += W, slot ^= 1) {
+        const uint8_t* sl = ring + slot * L::SLOT;
+        const int t0 = t_begin + L::T * j;
+        const bool next = j + W < n_tiles;
+        if (next) tf_kv8_wait<L::PER + L::COPIES>();
+        else tf_kv8_wait<L::COPIES>();
+        // ---- scores of tokens 16 u + 4 g + r
+        float sv[2][4];
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            float ksc[4][NG];
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const float* kp = reinterpret_cast<const float*>(sl + L::KDOFF) + (16 * u + 4 * g + r) * NG;
+#pragma unroll
+                for (int i = 0; i < NG; i++) ksc[r][i] = kp[i];
+            }
+            float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < NG; i++) {
+                const int row = 16 * u + n;
+                const tf_h16x8 kf = tf_i8_f16(*reinterpret_cast<const tf_u32x2*>(
+                    sl + L::KOFF + row * HD + 16 * ((2 * i + (g >> 1)) ^ L::kswz(row)) + 8 * (g & 1)));
+                tf_f32x4v c = tf_f32x4v{0.f, 0.f, 0.f, 0.f};
+                c = tf_mfma_f16_k32(kf, qa[i][1], c);
+                c = tf_mfma_f16_k32(kf, qa[i][0], c);
+#pragma unroll
+                for (int r = 0; r < 4; r++) acc[r] = fmaf(c[r], ksc[r][i], acc[r]);
+            }
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                float x = acc[r] * scale;
+                asm("" : "+v"(x));  // rounded before the maximum is subtracted
+                sv[u][r] = t0 + 16 * u + 4 * g + r < t_end ? x : -INFINITY;
             }
         }
-        __builtin_amdgcn_wave_barrier();
+        float vsc[2][4][NG], top = 0.f, tm = sv[0][0];
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const float* vp = reinterpret_cast<const float*>(sl + L::VDOFF) + (16 * u + 4 * g + r) * NG;
+#pragma unroll
+                for (int i = 0; i < NG; i++) {
+                    vsc[u][r][i] = vp[i];
+                    top = fmaxf(top, vsc[u][r][i]);
+                }
+                tm = fmaxf(tm, sv[u][r]);
+            }
+        if (__ballot(tm > m) | __ballot(top >= vtop)) {
+            tm = fmaxf(tm, __shfl_xor(tm, 16));
+            tm = fmaxf(tm, __shfl_xor(tm, 32));
+            top = fmaxf(vtop, tf_wave_max(top));
+            const float m_new = fmaxf(m, tm);
+            const float alpha = __expf(m - m_new);
+            // the power of two that takes scales up to `top` below 2^15
+            int fe = 141 - (int)(__float_as_uint(top) >> 23);
+            fe = fe > 126 ? 126 : fe < -126 ? -126 : fe;
+            const float f = __uint_as_float((uint32_t)(fe + 127) << 23);
+            // the first factor is whatever O = 0 takes
+            const float re = alpha * (vtop > 0.f ? f / vf : 1.f);
+            vf = f;
+            vtop = fe <= -113 ? INFINITY : __uint_as_float((uint32_t)(142 - fe) << 23);
+            m = m_new;
+            l *= alpha;
+#pragma unroll
+            for (int b = 0; b < DB; b++) o[b] *= re;
+        }
+        float p[2][4];
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                p[u][r] = __builtin_amdgcn_exp2f((sv[u][r] - m) * 1.44269504088896340736f);
+                l += p[u][r];
+                p[u][r] *= vf;
+            }
+        if (next) tf_kv8_wait<L::PER>();
+        else tf_kv8_wait<0>();
+        // ---- V^T P^T, a group of 32 dims at a time
+#pragma unroll
+        for (int i = 0; i < NG; i++) {
+            tf_h16x8 hi, lo;
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int r = 0; r < 4; r += 2) {
+                    tf_h2x h2, l2;
+                    tf_kv8_split(p[u][r] * vsc[u][r][i], p[u][r + 1] * vsc[u][r + 1][i], h2, l2);
+                    hi[4 * u + r] = h2.x, hi[4 * u + r + 1] = h2.y;
+                    lo[4 * u + r] = l2.x, lo[4 * u + r + 1] = l2.y;
+                }
+#pragma unroll
+            for (int b = 2 * i; b < 2 * i + 2; b++) {
+                typedef int i32x2 __attribute__((ext_vector_type(2)));
+                const tf_h16x8 va = tf_i8_f16(__builtin_bit_cast(
+                    tf_u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+                                  (__attribute__((address_space(3))) i32x2*)(sl + vbase + 16 * (b ^ vx)))));
+                o[b] = tf_mfma_f16_k32(va, lo, o[b]);
+                o[b] = tf_mfma_f16_k32(va, hi, o[b]);
+            }
+        }
+        if (j + 2 * W < n_tiles) {
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the slot has been read
+            issue(j + 2 * W, slot);
+        }
     }
-    float* base = partial + ((size_t)h * n_split + s) * (2 + HD);
-    if (lane == 0) {
-        base[0] = m;
-        base[1] = l;
+
+    // ---- merge the waves' (m, l, O)
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    __syncthreads();  // every wave is done with its ring
+    float* cmb = reinterpret_cast<float*>(lds);
+    const int nw = n_tiles < W ? n_tiles : W;
+    if (wave < nw) {
+        float* row = cmb + (wave * 16 + n) * L::CR;
+        if (g == 0) {
+            row[0] = m;
+            row[1] = l;
+        }
+        const float inv = 1.f / vf;  // a power of two
+#pragma unroll
+        for (int b = 0; b < DB; b++) *reinterpret_cast<tf_f32x4v*>(row + 4 + 16 * b + 4 * g) = o[b] * inv;
     }
-    for (int i = 0; i < DPL; i++) base[2 + lane + 64 * i] = o[i];
+    __syncthreads();
+    for (int i = tid; i < G * HD; i += 64 * W) {
+        const int h = i / HD, d = i % HD;
+        float M = TF_NEG_BIG;
+        for (int w = 0; w < nw; w++) M = fmaxf(M, cmb[(w * 16 + h) * L::CR]);
+        float O = 0.f, S = 0.f;
+        for (int w = 0; w < nw; w++) {
+            const float* row = cmb + (w * 16 + h) * L::CR;
+            const float a = __expf(row[0] - M);
+            O += a * row[4 + d];
+            S += a * row[1];
+        }
+        if (out) {  // workgroup-uniform; G * HD is a multiple of 64
+            const float v = O / fmaxf(S, 1e-20f);
+            const size_t oi = (size_t)kv_h * G * HD + i;
+            out[oi] = v;
+            if (q8) {  // this 32-lane half holds one 32-value group
+                const float amax = tf_group32_max(fabsf(v));
+                const float dq = amax * (1.0f / 127.0f);
+                q8[oi] = (int8_t)tf_q8_value(v, amax, dq);
+                if ((lane & 31) == 0) d8[oi >> 5] = dq;
+            }
+            continue;
+        }
+        float* base = partial + ((size_t)(kv_h * G + h) * n_split + s) * (2 + HD);
+        if (d == 0) {
+            base[0] = M;
+            base[1] = S;
+        }
+        base[2 + d] = O;
+    }
+}
+
+template <int HD>
+static int tf_flash_kv8_launch(const float* q, const int8_t* k8, const float* kd, const int8_t* v8,
+                               const float* vd, float* partial, int n_head, int n_kv, int pos0,
+                               const int* pos0_dev, int n_split, float scale, float* out,
+                               int8_t* q8, float* d8, tf_stream_t stream) {
+    using L = TfKv8<HD>;
+    // 4 bytes a copy for the scales of head_dim 64, else 16
+    const uintptr_t sc = (uintptr_t)kd | (uintptr_t)vd;
+    TF_CHECK_ARG((((uintptr_t)q | (uintptr_t)k8 | (uintptr_t)v8) & 15) == 0 &&
+                 (sc & (HD == 64 ? 3 : 15)) == 0);
+    const int rc = tf_set_lds_limit((const void*)tf_flash_kv8_kernel<HD>, L::LDS);
+    if (rc) return rc;
+    hipLaunchKernelGGL(tf_flash_kv8_kernel<HD>, dim3(n_kv, n_split), dim3(64 * L::W), L::LDS,
+                       tf_stream(stream), q, k8, kd, v8, vd, partial, n_head, n_kv, pos0, pos0_dev,
+                       n_split, scale, n_split == 1 ? out : nullptr, q8, d8);
+    return TF_LAUNCH_RESULT();
 }
 
 // ---------------------------------------------------------------- C ABI
@@ -170,19 +506,18 @@ extern "C" int tf_flash_decode_kv8(const float* q, const int8_t* k8, const float
     TF_CHECK_ARG(q && k8 && kd && v8 && vd && partial && out && ((q8 == nullptr) == (d8 == nullptr)));
     TF_CHECK_ARG(n_head > 0 && n_kv > 0 && n_head % n_kv == 0 && n_head / n_kv <= 16);
     TF_CHECK_ARG(n_split >= 1 && n_split <= 1024 && (pos0_dev || (pos0 >= 0 && pos0 < INT32_MAX - 1024)));
-    auto go = [&](auto kern) {
-        hipLaunchKernelGGL(kern, dim3((n_head + 3) / 4, n_split), dim3(256), 0, tf_stream(stream), q,
-                           k8, kd, v8, vd, partial, n_head, n_kv, pos0, pos0_dev, n_split, scale);
-        return TF_LAUNCH_RESULT();
+    auto go = [&](auto fn) {
+        return fn(q, k8, kd, v8, vd, partial, n_head, n_kv, pos0, pos0_dev, n_split, scale, out, q8,
+                  d8, stream);
     };
     int rc;
     switch (head_dim) {
-    case 64: rc = go(tf_flash_kv8_kernel<64>); break;
-    case 128: rc = go(tf_flash_kv8_kernel<128>); break;
-    case 256: rc = go(tf_flash_kv8_kernel<256>); break;
+    case 64: rc = go(tf_flash_kv8_launch<64>); break;
+    case 128: rc = go(tf_flash_kv8_launch<128>); break;
+    case 256: rc = go(tf_flash_kv8_launch<256>); break;
     default: return (int)hipErrorInvalidValue;
     }
-    if (rc) return rc;
+    if (rc || n_split == 1) return rc;
     return q8 ? tf_flash_decode_reduce_q8(partial, out, q8, d8, n_head, head_dim, n_split, stream)
               : tf_flash_decode_reduce(partial, out, n_head, head_dim, n_split, 1, stream);
 }
