@@ -159,23 +159,25 @@ template <int HD>
 __global__ __launch_bounds__(64 * TfKv8<HD>::W) void tf_flash_kv8_kernel(
     const float* __restrict__ q, const int8_t* __restrict__ k8, const float* __restrict__ kd,
     const int8_t* __restrict__ v8, const float* __restrict__ vd, float* __restrict__ partial,
-    int n_head, int n_kv, int pos0, const int* __restrict__ pos0_dev, int n_split, float scale,
+    int G, int n_kv, int pos0, const int* __restrict__ pos0_dev, int n_split, float scale,
     float* __restrict__ out, int8_t* __restrict__ q8, float* __restrict__ d8) {
     using L = TfKv8<HD>;
     constexpr int NG = L::NG, DB = L::DB, W = L::W;
     extern __shared__ __align__(16) uint8_t lds[];
-    const int kv_h = blockIdx.x, s = blockIdx.y, G = n_head / n_kv;
+    const int kv_h = blockIdx.y, s = blockIdx.x + 8 * blockIdx.z;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 15, g = lane >> 4;
     if (pos0_dev) pos0 = pos0_dev[0];
     const int seq = pos0 + 1;
     // whole tiles a split
-    const int chunk = (int)((((long long)seq + n_split - 1) / n_split + L::T - 1) / L::T * L::T);
-    const int t_begin = (int)min((long long)s * chunk, (long long)seq);
-    const int t_end = (int)min((long long)t_begin + chunk, (long long)seq);
-    const int n_tiles = (t_end - t_begin + L::T - 1) / L::T;
-    const size_t row8 = (size_t)n_kv * HD, rowd = (size_t)n_kv * NG * 4;
+    const uint32_t tiles = seq > 0 ? ((uint32_t)seq + L::T - 1) / L::T : 0;
+    const uint32_t share = (tiles + n_split - 1) / (uint32_t)n_split;
+    const uint32_t first = min(s * share, tiles);
+    const int n_tiles = (int)min(share, tiles - first);
+    const int t_begin = (int)first * L::T;
+    const int t_end = n_tiles ? min(t_begin + n_tiles * L::T, seq) : t_begin;
+    const uint32_t row8 = (uint32_t)n_kv * HD, rowd = (uint32_t)n_kv * NG * 4;  // bytes
     uint8_t* ring = lds + wave * 2 * L::SLOT;
 
     // the query's rows (heads past G repeat the last) into wave 0's second slot
@@ -188,38 +190,57 @@ __global__ __launch_bounds__(64 * TfKv8<HD>::W) void tf_flash_kv8_kernel(
             tf_lds_dma16(qk + (size_t)h * HD + 4 * (lane % (HD / 4)),
                          tf_lds_off(lds) + L::SLOT + 1024 * i);
         }
-    // tile j -> slot: K, the scales of K and V, V; rows past the split repeat its
-    // last (their weights are zero)
-    auto issue = [&](int j, int slot) {
+    // tile j -> slot: K and the scales of K and V (issue_k), then V (issue_v); rows
+    // past the split repeat its last (their weights are zero).  Offsets inside a tile
+    // are 24-bit products: row8 < 2^24.
+    constexpr int RPC = 64 / L::NC;  // rows of a copy
+    const int lr = lane / L::NC, lc = lane % L::NC;
+    auto k_off = [&](int i, int last) {
+        const int r = RPC * i + lr;
+        return __umul24(min(r, last), row8) + 16 * (lc ^ L::kswz(r));
+    };
+    auto v_off = [&](int i, int last) {
+        const int r = RPC * i + lr;
+        return __umul24(min(r, last), row8) + 16 * (lc ^ L::vswz(r));
+    };
+    auto s_off = [&](int last) {
+        const int l = HD == 128 ? lane & 31 : lane >> 1;
+        return __umul24(min(l, last), rowd) +
+               (HD == 128 ? 0 : (HD == 256 ? 16 : 4) * (lane & 1));
+    };
+    const uint8_t* k_head = reinterpret_cast<const uint8_t*>(k8) + kv_h * HD;
+    const uint8_t* v_head = reinterpret_cast<const uint8_t*>(v8) + kv_h * HD;
+    const uint8_t* kd_head = reinterpret_cast<const uint8_t*>(kd) + kv_h * NG * 4;
+    const uint8_t* vd_head = reinterpret_cast<const uint8_t*>(vd) + kv_h * NG * 4;
+    auto issue_k = [&](int j, int slot) {
         const int t0 = t_begin + L::T * j, last = t_end - 1 - t0;
         const uint32_t base = tf_lds_off(ring) + slot * L::SLOT;
-        const uint8_t* kb = reinterpret_cast<const uint8_t*>(k8) + (size_t)t0 * row8 + kv_h * HD;
-        const uint8_t* vb = reinterpret_cast<const uint8_t*>(v8) + (size_t)t0 * row8 + kv_h * HD;
-        const uint8_t* kdb = reinterpret_cast<const uint8_t*>(kd) + (size_t)t0 * rowd + kv_h * NG * 4;
-        const uint8_t* vdb = reinterpret_cast<const uint8_t*>(vd) + (size_t)t0 * rowd + kv_h * NG * 4;
-        constexpr int RPC = 64 / L::NC;  // rows of a copy
+        const uint8_t* kb = k_head + (size_t)t0 * row8;
+        const uint8_t* kdb = kd_head + (size_t)t0 * rowd;
+        const uint8_t* vdb = vd_head + (size_t)t0 * rowd;
 #pragma unroll
-        for (int i = 0; i < L::COPIES; i++) {
-            const int r = RPC * i + lane / L::NC, c = (lane % L::NC) ^ L::kswz(r);
-            tf_lds_dma16(kb + (size_t)min(r, last) * row8 + 16 * c, base + L::KOFF + 1024 * i);
-        }
+        for (int i = 0; i < L::COPIES; i++)
+            tf_lds_dma_s<16>(kb, k_off(i, last), base + L::KOFF + 1024 * i);
+        const uint32_t so = s_off(last);
         if constexpr (HD == 128) {
-            const int r = min(lane & 31, last);
-            tf_lds_dma16((lane < 32 ? kdb : vdb) + (size_t)r * rowd, base + L::KDOFF);
-        } else if constexpr (HD == 256) {
-            const size_t o = (size_t)min(lane >> 1, last) * rowd + 16 * (lane & 1);
-            tf_lds_dma16(kdb + o, base + L::KDOFF);
-            tf_lds_dma16(vdb + o, base + L::VDOFF);
+            tf_lds_dma16((lane < 32 ? kdb : vdb) + so, base + L::KDOFF);
         } else {
-            const uint32_t o = (uint32_t)(min(lane >> 1, last) * (int)rowd + 4 * (lane & 1));
-            tf_lds_dma_s<4>(kdb, o, base + L::KDOFF);
-            tf_lds_dma_s<4>(vdb, o, base + L::VDOFF);
+            constexpr int DW = HD == 256 ? 16 : 4;
+            tf_lds_dma_s<DW>(kdb, so, base + L::KDOFF);
+            tf_lds_dma_s<DW>(vdb, so, base + L::VDOFF);
         }
+    };
+    auto issue_v = [&](int j, int slot) {
+        const int t0 = t_begin + L::T * j, last = t_end - 1 - t0;
+        const uint32_t base = tf_lds_off(ring) + slot * L::SLOT;
+        const uint8_t* vb = v_head + (size_t)t0 * row8;
 #pragma unroll
-        for (int i = 0; i < L::COPIES; i++) {
-            const int r = RPC * i + lane / L::NC, c = (lane % L::NC) ^ L::vswz(r);
-            tf_lds_dma16(vb + (size_t)min(r, last) * row8 + 16 * c, base + L::VOFF + 1024 * i);
-        }
+        for (int i = 0; i < L::COPIES; i++)
+            tf_lds_dma_s<16>(vb, v_off(i, last), base + L::VOFF + 1024 * i);
+    };
+    auto issue = [&](int j, int slot) {
+        issue_k(j, slot);
+        issue_v(j, slot);
     };
     const bool any = wave < n_tiles;
     if (any) {
@@ -251,17 +272,19 @@ __global__ __launch_bounds__(64 * TfKv8<HD>::W) void tf_flash_kv8_kernel(
 #pragma unroll
             for (int i = 0; i < 8; i++) qmax = fmaxf(qmax, fabsf(qv[j][i]));
         qmax = tf_wave_max(qmax);
-        const int e = qmax > 0.f ? ilogbf(qmax) - 14 : 0;
+        int fe = 141 - (int)(__float_as_uint(qmax) >> 23);
+        fe = fe > 126 ? 126 : fe < -113 ? -113 : fe;
+        const float f = __uint_as_float((uint32_t)(fe + 127) << 23);
 #pragma unroll
         for (int j = 0; j < NG; j++)
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const float x = ldexpf(qv[j][i], -e);
-                const _Float16 h0 = (_Float16)x;
-                qa[j][0][i] = h0;
-                qa[j][1][i] = (_Float16)(x - (float)h0);
+            for (int i = 0; i < 8; i += 2) {
+                tf_h2x h2, l2;
+                tf_kv8_split(qv[j][i] * f, qv[j][i + 1] * f, h2, l2);
+                qa[j][0][i] = h2.x, qa[j][0][i + 1] = h2.y;
+                qa[j][1][i] = l2.x, qa[j][1][i + 1] = l2.y;
             }
-        scale = ldexpf(scale, e);
+        scale *= __uint_as_float((uint32_t)(127 - fe) << 23);
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();  // the query has been read: its slot is free
@@ -285,28 +308,44 @@ __global__ __launch_bounds__(64 * TfKv8<HD>::W) void tf_flash_kv8_kernel(
         const bool next = j + W < n_tiles;
         if (next) tf_kv8_wait<L::PER + L::COPIES>();
         else tf_kv8_wait<L::COPIES>();
+        // everything that the scores take, at once: the reads overlap, and the next tile's
+        // K can be on its way under all of the arithmetic
+        const bool refill = j + 2 * W < n_tiles;
+        tf_u32x2 kraw[2][NG];
+        float ksc[2][4][NG], vsc[2][4][NG];
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int i = 0; i < NG; i++) {
+                const int row = 16 * u + n;
+                kraw[u][i] = *reinterpret_cast<const tf_u32x2*>(
+                    sl + L::KOFF + row * HD + 16 * ((2 * i + (g >> 1)) ^ L::kswz(row)) + 8 * (g & 1));
+            }
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const int row = 16 * u + 4 * g + r;
+                const float* kp = reinterpret_cast<const float*>(sl + L::KDOFF) + row * NG;
+                const float* vp = reinterpret_cast<const float*>(sl + L::VDOFF) + row * NG;
+#pragma unroll
+                for (int i = 0; i < NG; i++) ksc[u][r][i] = kp[i], vsc[u][r][i] = vp[i];
+            }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        if (refill) issue_k(j + 2 * W, slot);
         // ---- scores of tokens 16 u + 4 g + r
         float sv[2][4];
 #pragma unroll
         for (int u = 0; u < 2; u++) {
-            float ksc[4][NG];
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const float* kp = reinterpret_cast<const float*>(sl + L::KDOFF) + (16 * u + 4 * g + r) * NG;
-#pragma unroll
-                for (int i = 0; i < NG; i++) ksc[r][i] = kp[i];
-            }
             float acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int i = 0; i < NG; i++) {
-                const int row = 16 * u + n;
-                const tf_h16x8 kf = tf_i8_f16(*reinterpret_cast<const tf_u32x2*>(
-                    sl + L::KOFF + row * HD + 16 * ((2 * i + (g >> 1)) ^ L::kswz(row)) + 8 * (g & 1)));
+                const tf_h16x8 kf = tf_i8_f16(kraw[u][i]);
                 tf_f32x4v c = tf_f32x4v{0.f, 0.f, 0.f, 0.f};
                 c = tf_mfma_f16_k32(kf, qa[i][1], c);
                 c = tf_mfma_f16_k32(kf, qa[i][0], c);
 #pragma unroll
-                for (int r = 0; r < 4; r++) acc[r] = fmaf(c[r], ksc[r][i], acc[r]);
+                for (int r = 0; r < 4; r++) acc[r] = fmaf(c[r], ksc[u][r][i], acc[r]);
             }
 #pragma unroll
             for (int r = 0; r < 4; r++) {
@@ -315,17 +354,13 @@ __global__ __launch_bounds__(64 * TfKv8<HD>::W) void tf_flash_kv8_kernel(
                 sv[u][r] = t0 + 16 * u + 4 * g + r < t_end ? x : -INFINITY;
             }
         }
-        float vsc[2][4][NG], top = 0.f, tm = sv[0][0];
+        float top = 0.f, tm = sv[0][0];
 #pragma unroll
         for (int u = 0; u < 2; u++)
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                const float* vp = reinterpret_cast<const float*>(sl + L::VDOFF) + (16 * u + 4 * g + r) * NG;
 #pragma unroll
-                for (int i = 0; i < NG; i++) {
-                    vsc[u][r][i] = vp[i];
-                    top = fmaxf(top, vsc[u][r][i]);
-                }
+                for (int i = 0; i < NG; i++) top = fmaxf(top, vsc[u][r][i]);
                 tm = fmaxf(tm, sv[u][r]);
             }
         if (__ballot(tm > m) | __ballot(top >= vtop)) {
@@ -356,34 +391,35 @@ __global__ __launch_bounds__(64 * TfKv8<HD>::W) void tf_flash_kv8_kernel(
                 l += p[u][r];
                 p[u][r] *= vf;
             }
-        if (next) tf_kv8_wait<L::PER>();
-        else tf_kv8_wait<0>();
-        // ---- V^T P^T, a group of 32 dims at a time
+        tf_h16x8 ph[NG], pl[NG];  // p vd[t][i], by group of dims
 #pragma unroll
-        for (int i = 0; i < NG; i++) {
-            tf_h16x8 hi, lo;
+        for (int i = 0; i < NG; i++)
 #pragma unroll
             for (int u = 0; u < 2; u++)
 #pragma unroll
                 for (int r = 0; r < 4; r += 2) {
                     tf_h2x h2, l2;
                     tf_kv8_split(p[u][r] * vsc[u][r][i], p[u][r + 1] * vsc[u][r + 1][i], h2, l2);
-                    hi[4 * u + r] = h2.x, hi[4 * u + r + 1] = h2.y;
-                    lo[4 * u + r] = l2.x, lo[4 * u + r + 1] = l2.y;
+                    ph[i][4 * u + r] = h2.x, ph[i][4 * u + r + 1] = h2.y;
+                    pl[i][4 * u + r] = l2.x, pl[i][4 * u + r + 1] = l2.y;
                 }
+        if (refill) tf_kv8_wait<L::PER + L::K_COPIES>();
+        else if (next) tf_kv8_wait<L::PER>();
+        else tf_kv8_wait<0>();
+        // ---- V^T P^T
+        typedef int i32x2 __attribute__((ext_vector_type(2)));
+        i32x2 vraw[DB];
 #pragma unroll
-            for (int b = 2 * i; b < 2 * i + 2; b++) {
-                typedef int i32x2 __attribute__((ext_vector_type(2)));
-                const tf_h16x8 va = tf_i8_f16(__builtin_bit_cast(
-                    tf_u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-                                  (__attribute__((address_space(3))) i32x2*)(sl + vbase + 16 * (b ^ vx)))));
-                o[b] = tf_mfma_f16_k32(va, lo, o[b]);
-                o[b] = tf_mfma_f16_k32(va, hi, o[b]);
-            }
-        }
-        if (j + 2 * W < n_tiles) {
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the slot has been read
-            issue(j + 2 * W, slot);
+        for (int b = 0; b < DB; b++)
+            vraw[b] = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+                (__attribute__((address_space(3))) i32x2*)(sl + vbase + 16 * (b ^ vx)));
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        if (refill) issue_v(j + 2 * W, slot);
+#pragma unroll
+        for (int b = 0; b < DB; b++) {
+            const tf_h16x8 va = tf_i8_f16(__builtin_bit_cast(tf_u32x2, vraw[b]));
+            o[b] = tf_mfma_f16_k32(va, pl[b / 2], o[b]);
+            o[b] = tf_mfma_f16_k32(va, ph[b / 2], o[b]);
         }
     }
 
@@ -448,9 +484,14 @@ static int tf_flash_kv8_launch(const float* q, const int8_t* k8, const float* kd
                  (sc & (HD == 64 ? 3 : 15)) == 0);
     const int rc = tf_set_lds_limit((const void*)tf_flash_kv8_kernel<HD>, L::LDS);
     if (rc) return rc;
-    hipLaunchKernelGGL(tf_flash_kv8_kernel<HD>, dim3(n_kv, n_split), dim3(64 * L::W), L::LDS,
-                       tf_stream(stream), q, k8, kd, v8, vd, partial, n_head, n_kv, pos0, pos0_dev,
-                       n_split, scale, n_split == 1 ? out : nullptr, q8, d8);
+    // Workgroup b runs on XCD b mod 8: where the splits divide by 8, the kv heads of
+    // one split, whose rows lie side by side, share an XCD and its L2 (8 kv heads, 302
+    // MB: 83 -> 71 us).
+    const bool eights = n_split % 8 == 0;
+    const dim3 grid(eights ? 8 : n_split, n_kv, eights ? n_split / 8 : 1);
+    hipLaunchKernelGGL(tf_flash_kv8_kernel<HD>, grid, dim3(64 * L::W), L::LDS, tf_stream(stream), q,
+                       k8, kd, v8, vd, partial, n_head / n_kv, n_kv, pos0, pos0_dev, n_split, scale,
+                       n_split == 1 ? out : nullptr, q8, d8);
     return TF_LAUNCH_RESULT();
 }
 
@@ -493,9 +534,19 @@ extern "C" int tf_kv8_read(const int8_t* k8, const float* kd, const int8_t* v8, 
     return TF_LAUNCH_RESULT();
 }
 
+// One split (and one launch) where it gives each wave at most one tile: 256 tokens
+// of 14/2 heads of 64 take 6.0 us against 7.1 in 8 splits, of 16/2 heads of 128 8.7
+// against 8.5.  Past that one for every 64 tokens, in eights for the XCDs, while the
+// workgroups fit the CUs at once (a second one has no LDS beside the first): 5001
+// tokens of 14/2 heads of 64 8.3 us in 64, 11 in 8; 131072 of 28/4 heads of 128 54 us
+// in 32, 40 in 64, 50 in 128.
 extern "C" int tf_flash_decode_kv8_n_split(int n_kv, int head_dim, int max_seq) {
-    (void)head_dim;
-    return tf_flash_decode_n_split(n_kv, max_seq);
+    if (n_kv <= 0 || max_seq <= (head_dim == 256 ? TfKv8<256>::W : TfKv8<128>::W) * TfKv8<128>::T)
+        return 1;
+    const int fit = tf_device_cus() / n_kv;
+    if (fit < 8) return fit > 0 ? fit : 1;
+    const int want = ((max_seq - 1) / 512 + 1) * 8;
+    return want < fit ? want : fit / 8 * 8;
 }
 
 extern "C" int tf_flash_decode_kv8(const float* q, const int8_t* k8, const float* kd,
@@ -505,7 +556,7 @@ extern "C" int tf_flash_decode_kv8(const float* q, const int8_t* k8, const float
                                    tf_stream_t stream) {
     TF_CHECK_ARG(q && k8 && kd && v8 && vd && partial && out && ((q8 == nullptr) == (d8 == nullptr)));
     TF_CHECK_ARG(n_head > 0 && n_kv > 0 && n_head % n_kv == 0 && n_head / n_kv <= 16);
-    TF_CHECK_ARG(n_split >= 1 && n_split <= 1024 && (pos0_dev || (pos0 >= 0 && pos0 < INT32_MAX - 1024)));
+    TF_CHECK_ARG(n_kv <= 65535 && n_split >= 1 && n_split <= 1024 && (pos0_dev || (pos0 >= 0 && pos0 < INT32_MAX - 1024)));
     auto go = [&](auto fn) {
         return fn(q, k8, kd, v8, vd, partial, n_head, n_kv, pos0, pos0_dev, n_split, scale, out, q8,
                   d8, stream);
