@@ -11,12 +11,27 @@
 // NaN and -inf are never drawn, +inf takes all the weight there is; T <= 0
 // takes the largest (lowest index); a row with nothing to draw gives 0.
 //
+// Weights and their sums are f64: with f32 sums of 10^5 weights the token
+// would depend on the order of addition for one u in a few thousand.  Where
+// sums are formed by atomics, weights are integers of 2^-46 of the largest (or
+// 2^-44, for a whole row), so that a sum has one value whatever the order.
+//
 // Every filter keeps a run from the front of one order, so what is kept is
-// named by its last element: a cut (key, number of elements kept that tie with
-// it, by index).  The cut is found by radix selection over the 32 bits of the
-// ordered logit, 8 bits a pass, by count for top-k and by weight for top-p;
-// no sort.  Weights are added as integers of 2^-44 of the largest, so that a
-// sum has one value whatever the order in which its atomics land.
+// named by its last element, and no row is sorted.  Three launches, rows cut
+// into chunks so that one row has the loads of many CUs:
+//   1. stats: a chunk's largest logit, and a histogram of counts and weights
+//      over bins of 1/16 of z below it (no filter: its sum of weights);
+//   2. gather: each chunk's workgroup adds the row's histograms, finds the bins
+//      in which the cuts of top-k and top-p lie, writes its elements of those
+//      bins to the row's list, and adds up the weights of the bins before them;
+//   3. draw: a workgroup a row takes the cuts from the list (radix selection
+//      in LDS, by count or weight), finds the chunk in which the running sum
+//      passes u, and walks that chunk.
+// Without top-k, top-p and min-p the second launch is left out.  A row whose
+// cut lies among more elements than the list holds (near-equal logits by the
+// ten thousand), or whose logits the bins cannot hold (an infinite one, T below
+// 1e-6), is selected by radix passes over the row itself in the third launch:
+// the same cut, found by one workgroup.
 #include <math.h>
 
 #include "tf_common.hpp"
@@ -26,6 +41,18 @@ namespace {
 
 typedef unsigned long long u64;
 
+constexpr int kBins = 512;          // of 1/16 of z: 32 below a chunk's largest, the last open
+constexpr float kPerZ = 16.f;
+constexpr int kList = 8192;         // elements of a row's list
+constexpr int kChunkThreads = 512, kChunkWaves = kChunkThreads / 64;
+constexpr int kBlock = 16 * kChunkThreads;  // elements that a chunk's workgroup holds at once
+constexpr int kMaxVocab = 1 << 19;
+constexpr int kMaxChunks = kMaxVocab / kBlock;  // 64
+constexpr int kRowThreads = 1024, kRowWaves = kRowThreads / 64;
+// Integer weights: a chunk has at most 2^17 elements, a row fewer than 2^19, so that
+// their sums stay below 2^63.
+constexpr double kChunkUnit = 0x1p46, kRowUnit = 0x1p44;
+
 // Ordered bits of a logit: NaN lowest, -0 as +0.
 __device__ __forceinline__ uint32_t order_key(float l) {
     if (l != l) return 0;
@@ -33,6 +60,10 @@ __device__ __forceinline__ uint32_t order_key(float l) {
     const uint32_t u = __float_as_uint(l);
     return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
+__device__ __forceinline__ float key_logit(uint32_t k) {
+    return __uint_as_float((k & 0x80000000u) ? k ^ 0x80000000u : ~k);
+}
+constexpr uint32_t kKeyMinusInf = 0x007fffffu;
 
 struct SampleArgs {
     const float* logits;
@@ -44,226 +75,723 @@ struct SampleArgs {
     const float* min_p;
     const float* u;
     int* out;
+    int chunk, chunks;  // elements of a chunk, chunks of a row
+    uint8_t* ws;
+    long long row_bytes;  // of the workspace
 };
 
-// What turns a logit of a row into its weight.
+// A row's workspace.
+struct RowInfo {
+    int lo, hi, k_bin;          // listed bins: lo .. hi, and k_bin
+    int k_before;               // elements in bins before k_bin
+    u64 w_before_k, w_before_lo, w_all;  // weights in bins before k_bin, before lo, in all
+    int cut;                    // 0: no cut, kept is what min-p keeps; 1: the list; 2: the row itself
+    int use_k;                  // top-k cuts something
+};
+struct ChunkStat {
+    float top;    // the largest logit
+    int index;    // its lowest index (T <= 0 only)
+    double sum;   // weights: of the chunk (no filter; of its largest), or kept for sure (of the row's)
+};
+__device__ __forceinline__ RowInfo* row_info(const SampleArgs& a, int row) {
+    return reinterpret_cast<RowInfo*>(a.ws + row * a.row_bytes);
+}
+__device__ __forceinline__ int* row_count(const SampleArgs& a, int row) {
+    return reinterpret_cast<int*>(a.ws + row * a.row_bytes + 120);
+}
+__device__ __forceinline__ u64* row_list(const SampleArgs& a, int row) {
+    return reinterpret_cast<u64*>(a.ws + row * a.row_bytes + 128);
+}
+__device__ __forceinline__ ChunkStat* row_stats(const SampleArgs& a, int row) {
+    return reinterpret_cast<ChunkStat*>(row_list(a, row) + kList);
+}
+__device__ __forceinline__ u64* chunk_weights(const SampleArgs& a, int row, int c) {
+    return reinterpret_cast<u64*>(row_stats(a, row) + a.chunks) + (size_t)c * (kBins + kBins / 2);
+}
+__device__ __forceinline__ uint32_t* chunk_counts(const SampleArgs& a, int row, int c) {
+    return reinterpret_cast<uint32_t*>(chunk_weights(a, row, c) + kBins);
+}
+static_assert(sizeof(RowInfo) <= 120, "the list's count follows");
+
+struct Settings {
+    float temp;
+    bool greedy, use_k, use_p, bad;
+    int k;
+    float p;
+    double min_w;
+    float per_l;  // bins a unit of logit
+    __device__ bool filtered() const { return use_k || use_p; }
+    __device__ bool plain() const { return !use_k && !use_p && !(min_w > 0.0); }
+};
+__device__ __forceinline__ Settings settings(const SampleArgs& a, int row) {
+    Settings s;
+    s.temp = a.temperature ? a.temperature[row] : 1.f;
+    s.greedy = !(s.temp > 0.f);
+    s.k = a.top_k ? a.top_k[row] : 0;
+    s.use_k = s.k > 0 && s.k < a.n;
+    s.p = a.top_p ? a.top_p[row] : 1.f;
+    s.use_p = s.p < 1.f;
+    const float m = a.min_p ? a.min_p[row] : 0.f;
+    s.min_w = m > 0.f ? fmin((double)m, 1.0) : 0.0;
+    s.per_l = kPerZ / s.temp;
+    s.bad = !(s.temp >= 1e-6f);
+    return s;
+}
+// Whether the bins can hold a row with this largest logit.
+__device__ __forceinline__ bool no_bins(const Settings& s, float l_max) {
+    return s.bad || !(fabsf(l_max) * s.per_l < 1e9f);
+}
+// The bin of a logit, counted from that of `base`; both by the same monotone product.
+__device__ __forceinline__ float bin_of(float l, float per_l) { return floorf(l * per_l); }
+__device__ __forceinline__ int bin_below(float base, float b) {
+    return (int)fminf(fmaxf(base - b, 0.f), (float)(kBins - 1));
+}
+
+// 2^y for y <= 0, to 2^-51: y is a multiple of 1/32 (read off the low bits of y plus
+// 1.5 * 2^47) and a rest below 1/64, whose series ends at the 6th power (the next term
+// is 2^-58), times 2^(j/32) from a table and the exponent.  NaN and what lies below
+// 2^-1000 give 0.  Some twenty instructions where exp() takes sixty; a row calls it for
+// every token.
+__constant__ double kExp2Table[32] = {
+    1, 1.0218971486541166, 1.0442737824274138, 1.0671404006768237,
+    1.0905077326652577, 1.1143867425958924, 1.1387886347566916, 1.1637248587775775,
+    1.189207115002721, 1.215247359980469, 1.241857812073484, 1.2690509571917332,
+    1.2968395546510096, 1.3252366431597413, 1.3542555469368927, 1.383909881963832,
+    1.4142135623730951, 1.4451808069770467, 1.4768261459394993, 1.5091644275934228,
+    1.5422108254079407, 1.5759808451078865, 1.6104903319492543, 1.6457554781539649,
+    1.681792830507429, 1.7186192981224779, 1.7562521603732995, 1.7947090750031072,
+    1.8340080864093424, 1.8741676341103, 1.9152065613971474, 1.9571441241754002};
+__device__ __forceinline__ void fill_exp2(double* table) {
+    if (threadIdx.x < 32) table[threadIdx.x] = kExp2Table[threadIdx.x];
+}
+__device__ __forceinline__ double exp2_neg(double y, const double* table) {
+    constexpr double kShift = 0x1.8p47, ln2 = 0.69314718055994530942;
+    constexpr double c2 = ln2 * ln2 / 2, c3 = c2 * ln2 / 3, c4 = c3 * ln2 / 4, c5 = c4 * ln2 / 5,
+                     c6 = c5 * ln2 / 6;
+    const double t = y + kShift;
+    const int k = (int)(uint32_t)__builtin_bit_cast(u64, t);
+    const double f = y - (t - kShift);
+    double r = c6;
+    r = fma(r, f, c5);
+    r = fma(r, f, c4);
+    r = fma(r, f, c3);
+    r = fma(r, f, c2);
+    r = fma(r, f, ln2);
+    r = fma(r, f, 1.0);
+    r *= table[k & 31];
+    const u64 bits = __builtin_bit_cast(u64, r) + ((u64)(uint32_t)(k >> 5 << 20) << 32);
+    return y >= -1000.0 ? __builtin_bit_cast(double, bits) : 0.0;
+}
+
+// The running sum at which top-p is reached: p of a sum of weights, at least the first.
+__device__ __forceinline__ u64 p_goal(const Settings& s, u64 all) {
+    const double goal = s.p > 0.f ? ceil((double)s.p * (double)all) : 0.0;
+    return goal >= 1.0 ? (u64)goal : 1;
+}
+
+// What turns a logit of a row into its weight: exp((l - l_max) / T).
 struct RowWeight {
-    double t, z_max;
+    const double* table;
+    double per_t, l_max;  // per_t: powers of two a unit of logit
     bool inf;
+    __device__ RowWeight(const double* table_, float temp, float l_max_) {
+        table = table_;
+        per_t = 1.44269504088896340736 / (double)temp;
+        inf = l_max_ == INFINITY;
+        l_max = (double)l_max_;
+    }
     __device__ double operator()(float l) const {
         if (inf) return l == INFINITY ? 1.0 : 0.0;
-        return l > -INFINITY ? exp((double)l / t - z_max) : 0.0;  // NaN: 0
+        // T = inf: -inf times 0 is NaN and gives 0
+        return exp2_neg(((double)l - l_max) * per_t, table);
     }
 };
-
-constexpr int kThreads = 1024, kWaves = kThreads / 64;
-constexpr double kUnit = 0x1p44;  // integer weights; n < 2^19 keeps their sum below 2^63
-
-struct Cut {
-    uint32_t key;  // the last element's
-    int ties;      // elements with this key that are kept, lowest indices first
-};
+// The nearest integer to w / 2^-46 (2^-44) for w in [0, 1]: the low bits of w plus the
+// power of two with that last bit.
+__device__ __forceinline__ u64 chunk_units(double w) {
+    return __builtin_bit_cast(u64, w + 64.0) - __builtin_bit_cast(u64, 64.0);
+}
+__device__ __forceinline__ u64 row_units(double w) {
+    return __builtin_bit_cast(u64, w + 256.0) - __builtin_bit_cast(u64, 256.0);
+}
 
 __device__ __forceinline__ double wave_sum(double v) {
     for (int off = 32; off; off >>= 1) v += __shfl_xor(v, off, 64);
     return v;
 }
 
-// The cut of the element at which the running total, in falling order, reaches
-// `target` (1 <= target <= the total): of counts, or of integer weights.
-// Elements outside `within` are not there.
-template <bool WEIGHTS>
-__device__ Cut radix_cut(const float* x, int n, const RowWeight& w, Cut within, u64 target,
-                         u64* hist /* 256, LDS */, u64* share /* 2, LDS */) {
-    const int tid = threadIdx.x;
-    uint32_t prefix = 0;
-    u64 each = 1, tied = 0;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        if (tid < 256) hist[tid] = 0;
-        __syncthreads();
-        const uint32_t mask = shift == 24 ? 0u : ~0u << (shift + 8);
-        for (int i = tid; i < n; i += kThreads) {
-            const uint32_t key = order_key(x[i]);
-            if ((key & mask) != prefix || key < within.key) continue;
-            // the elements that tie with `within` count for what is kept of them: below
-            if (key == within.key) continue;
-            atomicAdd(&hist[(key >> shift) & 255],
-                      WEIGHTS ? (u64)(w(x[i]) * kUnit + 0.5) : (u64)1);
+// Elements i0 + 4 * tid + 2048 j + 0 .. 3 of a row; past `end`: -inf.
+__device__ __forceinline__ void load_block(const float* x, int i0, int end, float (&v)[16]) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const int i = i0 + 4 * (int)threadIdx.x + 4 * kChunkThreads * j;
+        if (i + 3 < end) {
+            const tf_u32x4 b = tf_ld16_a4(x + i);
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[4 * j + e] = __uint_as_float(b[e]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[4 * j + e] = i + e < end ? x[i + e] : -INFINITY;
         }
-        __syncthreads();
-        if (tid == 0) {
-            if (within.ties > 0 && (within.key & mask) == prefix) {
-                const float l = __uint_as_float((within.key & 0x80000000u) ? within.key ^ 0x80000000u
-                                                                            : ~within.key);
-                hist[(within.key >> shift) & 255] +=
-                    (u64)within.ties * (WEIGHTS ? (u64)(w(l) * kUnit + 0.5) : (u64)1);
-            }
-            int b = 255;
-            while (b > 0 && hist[b] < target) target -= hist[b--];
-            share[0] = target;
-            share[1] = (u64)b;
-        }
-        __syncthreads();
-        target = share[0];
-        prefix |= (uint32_t)share[1] << shift;
-        tied = hist[share[1]];
-        __syncthreads();
     }
-    if (WEIGHTS) {
-        const float l = __uint_as_float((prefix & 0x80000000u) ? prefix ^ 0x80000000u : ~prefix);
-        each = (u64)(w(l) * kUnit + 0.5);
-    }
-    // the first tie that reaches the target; a weight that rounds to nothing keeps them all
-    u64 need = each ? (target + each - 1) / each : (u64)n;
-    if (need < 1) need = 1;
-    if (need > (u64)n) need = (u64)n;
-    (void)tied;
-    return {prefix, (int)need};
+}
+__device__ __forceinline__ int block_index(int i0, int e) {
+    return i0 + 4 * (int)threadIdx.x + 4 * kChunkThreads * (e >> 2) + (e & 3);
 }
 
-__global__ __launch_bounds__(kThreads) void tf_sample_row_kernel(SampleArgs a) {
-    __shared__ u64 hist[256], share[2];
-    __shared__ double wave_w[kWaves], found_w;
-    __shared__ int wave_n[kWaves], first_max, answer;
+__global__ __launch_bounds__(kChunkThreads) void tf_sample_stats_kernel(SampleArgs a) {
+    __shared__ u64 weight[kBins];
+    __shared__ uint32_t count[kBins];
+    __shared__ double table[32], dpart[kChunkWaves];
+    __shared__ float part[kChunkWaves];
+    __shared__ int first;
+    const int row = blockIdx.x / a.chunks, c = blockIdx.x - row * a.chunks;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const float* x = a.logits + (size_t)row * a.stride;
+    const int i0 = c * a.chunk, end = min(i0 + a.chunk, a.n);
+    const bool many = end - i0 > kBlock;  // workgroup-uniform: the values are read again
+    float v[16];
+    load_block(x, i0, end, v);
+    const Settings s = settings(a, row);
+    fill_exp2(table);
+    for (int i = tid; i < kBins; i += kChunkThreads) weight[i] = 0, count[i] = 0;
+    if (tid == 0) first = a.n;
+    float top = -INFINITY;  // fmaxf passes NaN by
+#pragma unroll
+    for (int e = 0; e < 16; e++) top = fmaxf(top, v[e]);
+    for (int b = i0 + kBlock; b < end; b += kBlock) {
+        load_block(x, b, end, v);
+#pragma unroll
+        for (int e = 0; e < 16; e++) top = fmaxf(top, v[e]);
+    }
+    top = tf_wave_max(top);
+    if (lane == 0) part[wave] = top;
+    __syncthreads();
+    for (int i = 0; i < kChunkWaves; i++) top = fmaxf(top, part[i]);
+    ChunkStat* stat = row_stats(a, row) + c;
+    if (c == 0 && tid == 0) *row_count(a, row) = 0;
+    if (tid == 0) stat->top = top;
+    const bool empty = !(top > -INFINITY);
+    if (s.greedy) {
+        for (int i = i0 + tid; i < end; i += kChunkThreads)
+            if (x[i] == top) {
+                atomicMin(&first, i);
+                break;
+            }
+        __syncthreads();
+        if (tid == 0) stat->index = first;
+        return;
+    }
+    if (!s.filtered() && !s.plain()) return;
+    const RowWeight w(table, s.temp, top);
+    if (s.plain()) {
+        double sum = 0.0;
+        for (int b = i0; b < end && !empty; b += kBlock) {
+            if (many) load_block(x, b, end, v);
+#pragma unroll
+            for (int e = 0; e < 16; e++) sum += w(v[e]);
+        }
+        sum = wave_sum(sum);
+        if (lane == 0) dpart[wave] = sum;
+        __syncthreads();
+        if (tid == 0) {
+            for (int i = 1; i < kChunkWaves; i++) sum += dpart[i];
+            stat->sum = sum;
+        }
+        return;
+    }
+    if (!empty && !s.bad) {
+        const float base = bin_of(top, s.per_l);
+        for (int b = i0; b < end; b += kBlock) {
+            if (many) load_block(x, b, end, v);
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                if (!(v[e] > -INFINITY)) continue;  // NaN too
+                const int bin = bin_below(base, bin_of(v[e], s.per_l));
+                atomicAdd(&count[bin], 1u);
+                if (s.use_p) atomicAdd(&weight[bin], chunk_units(w(v[e])));
+            }
+        }
+    }
+    __syncthreads();
+    u64* gw = chunk_weights(a, row, c);
+    uint32_t* gc = chunk_counts(a, row, c);
+    for (int i = tid; i < kBins; i += kChunkThreads) gw[i] = weight[i], gc[i] = count[i];
+}
+
+// Inclusive scan over the workgroup (kChunkThreads threads), in thread order.
+template <class T>
+__device__ __forceinline__ T block_scan(T v, T* part /* kChunkWaves, LDS */) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int off = 1; off < 64; off <<= 1) {
+        const T o = __shfl_up(v, off, 64);
+        if (lane >= off) v += o;
+    }
+    if (lane == 63) part[wave] = v;
+    __syncthreads();
+    T before = 0;
+    for (int i = 0; i < wave; i++) before += part[i];
+    __syncthreads();
+    return v + before;
+}
+
+__global__ __launch_bounds__(kChunkThreads) void tf_sample_gather_kernel(SampleArgs a) {
+    __shared__ u64 w_upto[kBins], wpart[kChunkWaves];
+    __shared__ int n_upto[kBins], ipart[kChunkWaves];
+    __shared__ double table[32], dpart[kChunkWaves], chunk_f[kMaxChunks];
+    __shared__ int chunk_shift[kMaxChunks], first[3], share;
+    const int row = blockIdx.x / a.chunks, c = blockIdx.x - row * a.chunks;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const float* x = a.logits + (size_t)row * a.stride;
+    const int i0 = c * a.chunk, end = min(i0 + a.chunk, a.n);
+    const bool many = end - i0 > kBlock;  // workgroup-uniform
+    float v[16];
+    load_block(x, i0, end, v);
+    const Settings s = settings(a, row);
+    float mine_top = -INFINITY;
+    if (lane < a.chunks) mine_top = row_stats(a, row)[lane].top;
+    fill_exp2(table);
+    if (s.greedy || s.plain()) return;
+    const float l_max = tf_wave_max(mine_top);
+    if (!(l_max > -INFINITY)) return;
+    RowInfo info{};
+    if (s.filtered() && no_bins(s, l_max)) {
+        info.cut = 2;
+        if (c == 0 && tid == 0) *row_info(a, row) = info;
+        return;
+    }
+    const float base = bin_of(l_max, s.per_l);
+    w_upto[tid] = 0;
+    n_upto[tid] = 0;
+    if (tid < 3) first[tid] = kBins - 1;
+    __syncthreads();  // the table
+    const RowWeight w(table, s.temp, l_max);
+    int lo = kBins, hi = -1, k_bin = -1;  // min-p alone: every bin is kept for sure
+    if (s.filtered()) {
+        // bin b of the row: the chunks' bins, shifted by how far their largest lies below
+        // the row's, and their weights scaled alike; what falls past the last bin goes
+        // there.  Eight chunks' loads at once: one after the other they were half the time.
+        if (wave == 0) {
+            const bool any = mine_top > -INFINITY;
+            chunk_f[lane] = any ? w(mine_top) * (kRowUnit / kChunkUnit) : 0.0;
+            chunk_shift[lane] = any ? bin_below(base, bin_of(mine_top, s.per_l)) : 0;
+        }
+        __syncthreads();
+        for (int c8 = 0; c8 < a.chunks; c8 += 8) {
+            uint32_t nc[8];
+            u64 nw[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const int cc = min(c8 + i, a.chunks - 1);
+                nc[i] = chunk_counts(a, row, cc)[tid];
+                nw[i] = s.use_p ? chunk_weights(a, row, cc)[tid] : 0;
+            }
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                if (c8 + i >= a.chunks || nc[i] == 0) continue;
+                const int b = min(tid + chunk_shift[c8 + i], kBins - 1);
+                atomicAdd(&n_upto[b], (int)nc[i]);
+                if (s.use_p) atomicAdd(&w_upto[b], (u64)((double)nw[i] * chunk_f[c8 + i] + 0.5));
+            }
+        }
+        __syncthreads();
+        const u64 wt = block_scan(w_upto[tid], wpart);
+        const int nt = block_scan(n_upto[tid], ipart);
+        w_upto[tid] = wt;
+        n_upto[tid] = nt;
+        __syncthreads();
+        const bool use_k = s.use_k && n_upto[kBins - 1] > s.k;
+        if (use_k && nt >= s.k && (tid == 0 || n_upto[tid - 1] < s.k)) first[0] = tid;
+        __syncthreads();
+        info.use_k = use_k;
+        if (use_k) {
+            k_bin = first[0];
+            info.k_before = k_bin ? n_upto[k_bin - 1] : 0;
+            info.w_before_k = k_bin ? w_upto[k_bin - 1] : 0;
+            lo = hi = k_bin;
+        }
+        info.w_all = w_upto[kBins - 1];
+        if (s.use_p) {
+            // the goal is p of what top-k keeps: between these two until k_bin is resolved
+            auto reach = [&](u64 all, int slot) {
+                const u64 goal = p_goal(s, all);
+                if (wt >= goal && (tid == 0 || w_upto[tid - 1] < goal)) first[slot] = tid;
+            };
+            reach(use_k ? info.w_before_k : info.w_all, 1);
+            reach(use_k ? w_upto[k_bin] : info.w_all, 2);
+            __syncthreads();
+            lo = first[1];
+            hi = first[2];
+            if (use_k) lo = min(lo, k_bin), hi = min(hi, k_bin);
+        }
+        if (!use_k && !s.use_p) {
+            lo = kBins, hi = -1;
+        } else {
+            info.cut = 1;
+            info.w_before_lo = lo ? w_upto[lo - 1] : 0;
+            auto in_bins = [&](int b0, int b1) { return n_upto[b1] - (b0 ? n_upto[b0 - 1] : 0); };
+            const int listed = in_bins(lo, hi) + (k_bin > hi ? in_bins(k_bin, k_bin) : 0);
+            // min-p above the first listed bin (by a bin and the rounding of the bins'
+            // products): the cuts are past it
+            if (fabsf(base) < 1e5f && s.min_w > exp((2 - lo) * (1.0 / kPerZ))) {
+                info.cut = 0;
+                lo = kBins, hi = -1, k_bin = -1;
+            } else if (listed > kList) {
+                info.cut = 2;
+            }
+        }
+    }
+    info.lo = lo, info.hi = hi, info.k_bin = k_bin;
+    if (c == 0 && tid == 0) *row_info(a, row) = info;
+    if (info.cut == 2) return;
+    // the chunk's weight before bin lo, and its part of the list
+    double sum = 0.0;
+    for (int b = i0; b < end; b += kBlock) {
+        if (many) load_block(x, b, end, v);
+        uint32_t mine = 0;
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+            if (!(v[e] > -INFINITY)) continue;
+            const int bin = bin_below(base, bin_of(v[e], s.per_l));
+            if (bin < lo) {
+                const double we = w(v[e]);
+                sum += we >= s.min_w ? we : 0.0;
+            } else if (bin <= hi || bin == k_bin) {
+                mine |= 1u << e;
+            }
+        }
+        if (hi < 0) continue;  // workgroup-uniform
+        const int have = __popc(mine);
+        const int upto = block_scan(have, ipart);
+        if (tid == kChunkThreads - 1) share = upto ? atomicAdd(row_count(a, row), upto) : 0;
+        __syncthreads();
+        int at = share + upto - have;
+        u64* list = row_list(a, row);
+#pragma unroll
+        for (int e = 0; e < 16; e++)
+            if (mine >> e & 1 && at < kList)
+                list[at++] = (u64)order_key(v[e]) << 32 | (uint32_t)block_index(b, e);
+        __syncthreads();
+    }
+    sum = wave_sum(sum);
+    __syncthreads();
+    if (lane == 0) dpart[wave] = sum;
+    __syncthreads();
+    if (tid == 0) {
+        for (int i = 1; i < kChunkWaves; i++) sum += dpart[i];
+        row_stats(a, row)[c].sum = sum;
+    }
+}
+
+// ------------------------------------------------------------------ the cut
+
+struct Cut {
+    uint32_t key;  // the last kept element's: kept are larger ones,
+    int index;     // and equal ones up to this index
+    __device__ bool keeps(uint32_t k, int i) const { return k > key || (k == key && i <= index); }
+    // a cut found among what `outer` keeps: all of its equals are those that outer keeps
+    __device__ void within(const Cut& outer) {
+        if (key == outer.key) index = min(index, outer.index);
+    }
+};
+
+// LDS of a selection.
+struct Select {
+    u64 hist[256];
+    u64 left;
+    int digit;
+};
+
+// The largest digit d such that the total of digits >= d reaches s.left, which
+// is reduced by the total of those above it (0 if none reaches it); wave 0.
+__device__ __forceinline__ void pick_digit(Select& s) {
+    const int lane = threadIdx.x;
+    u64 h[4], sum = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) sum += h[i] = s.hist[255 - (4 * lane + i)];
+    u64 upto = sum;
+    for (int off = 1; off < 64; off <<= 1) {
+        const u64 o = __shfl_up(upto, off, 64);
+        if (lane >= off) upto += o;
+    }
+    const u64 left = s.left, over = __ballot(upto >= left);
+    const int who = over ? __builtin_ctzll(over) : 63;
+    if (lane == who) {
+        u64 run = upto - sum;
+        int i = 0;
+        while (i < 3 && run + h[i] < left) run += h[i++];
+        s.digit = 255 - (4 * lane + i);
+        s.left = left - run;
+    }
+}
+
+// The cut of the element at which the running total of `value`, in falling order
+// of key and rising order of index, reaches `goal` (of the elements that `each`
+// visits: each(f) calls f(key, index) for the thread's share).  `value(key)` is
+// an element's part of the total.
+template <class Each, class Value>
+__device__ Cut select_cut(Select& s, u64 goal, Each each, Value value) {
+    const int tid = threadIdx.x;
+    auto pass = [&](auto digit_of) {  // digit_of(key, index) < 0: not among them
+        __syncthreads();
+        if (tid < 256) s.hist[tid] = 0;
+        __syncthreads();
+        each([&](uint32_t key, int index) {
+            const int d = digit_of(key, index);
+            if (d >= 0) atomicAdd(&s.hist[d], value(key));
+        });
+        __syncthreads();
+        if (tid < 64) pick_digit(s);
+        __syncthreads();
+        return s.digit;
+    };
+    if (tid == 0) s.left = goal > 0 ? goal : 1;
+    uint32_t prefix = 0;
+    for (int shift = 24; shift >= 0; shift -= 8) {
+        const uint32_t mask = shift == 24 ? 0u : ~0u << (shift + 8);
+        prefix |= (uint32_t)pass([&](uint32_t key, int) {
+                      return (key & mask) == prefix ? (int)(key >> shift & 255) : -1;
+                  })
+                  << shift;
+    }
+    // equal elements share the total: how many of them, and which index is the last
+    const u64 each_value = value(prefix), left = s.left;
+    const u64 need = each_value ? (left + each_value - 1) / each_value : ~0ull;
+    __syncthreads();
+    if (tid == 0) s.hist[0] = 0;
+    __syncthreads();
+    u64 mine = 0;
+    each([&](uint32_t key, int) { mine += key == prefix; });
+    if (mine) atomicAdd(&s.hist[0], mine);
+    __syncthreads();
+    if (need >= s.hist[0]) return {prefix, kMaxVocab};
+    __syncthreads();
+    // the need-th lowest index: digits of its complement, so that falling order is rising
+    if (tid == 0) s.left = need * each_value;
+    uint32_t at = 0;
+    for (int shift = 16; shift >= 0; shift -= 8) {
+        const uint32_t mask = ~0u << (shift + 8) & 0xffffffu;
+        at |= (uint32_t)pass([&](uint32_t key, int index) {
+                  const uint32_t r = ~(uint32_t)index & 0xffffffu;
+                  return key == prefix && (r & mask) == at ? (int)(r >> shift & 255) : -1;
+              })
+              << shift;
+    }
+    return {prefix, (int)(~at & 0xffffffu)};
+}
+
+__global__ __launch_bounds__(kRowThreads) void tf_sample_draw_kernel(SampleArgs a) {
+    extern __shared__ __align__(16) uint8_t lds[];
+    u64* list = reinterpret_cast<u64*>(lds);                        // kList
+    u64* chunk_add = list + kList;                                  // kMaxChunks
+    Select& sel = *reinterpret_cast<Select*>(chunk_add + kMaxChunks);
+    __shared__ double wave_w[kRowWaves], table[32];
+    __shared__ u64 total_w;
+    __shared__ int answer;
     const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const float* x = a.logits + (size_t)row * a.stride;
     const int n = a.n;
-
-    // the largest logit, and the lowest index that has it
-    uint32_t top = 0;
-    for (int i = tid; i < n; i += kThreads) top = max(top, order_key(x[i]));
-    for (int off = 32; off; off >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, off, 64));
-    if (lane == 0) wave_n[wave] = (int)top;
-    if (tid == 0) first_max = n, answer = -1;
-    __syncthreads();
-    for (int i = 0; i < kWaves; i++) top = max(top, (uint32_t)wave_n[i]);
-    for (int i = tid; i < n; i += kThreads)
-        if (order_key(x[i]) == top) {
-            atomicMin(&first_max, i);
-            break;
-        }
-    __syncthreads();
-    const float l_max = __uint_as_float((top & 0x80000000u) ? top ^ 0x80000000u : ~top);
-    const float temp = a.temperature ? a.temperature[row] : 1.f;
-    if (top <= 0x007fffffu) {  // all NaN or -inf
-        if (tid == 0) a.out[row] = 0;
+    // everything that the workspace may hold of the row, at once
+    const Settings s = settings(a, row);
+    ChunkStat mine_c{-INFINITY, 0, 0.0};
+    if (lane < a.chunks) mine_c = row_stats(a, row)[lane];
+    RowInfo info = *row_info(a, row);
+    if (s.plain()) info.cut = 0;
+    const int count = min(*row_count(a, row), kList);
+    fill_exp2(table);
+    const float l_max = tf_wave_max(mine_c.top);
+    if (!(l_max > -INFINITY) || s.greedy) {  // nothing to draw, or nothing to choose
+        const u64 has = __ballot(lane < a.chunks && mine_c.top == l_max);
+        const int index = __shfl(mine_c.index, has ? __builtin_ctzll(has) : 0, 64);
+        if (tid == 0) a.out[row] = l_max > -INFINITY ? index : 0;
         return;
     }
-    if (!(temp > 0.f)) {
-        if (tid == 0) a.out[row] = first_max;
-        return;
-    }
-    RowWeight w;
-    w.t = (double)temp;
-    w.inf = l_max == INFINITY;
-    w.z_max = (double)l_max / w.t;
+    const RowWeight w(table, s.temp, l_max);
+    auto units = [&](uint32_t key) { return row_units(w(key_logit(key))); };
+    auto one = [](uint32_t) { return (u64)1; };
+    if (tid == 0) answer = -1, total_w = 0;
+    if (tid < kMaxChunks) chunk_add[tid] = 0;
+    __syncthreads();
 
-    Cut cut{0u, n};  // everything
-    const int k = a.top_k ? a.top_k[row] : 0;
-    if (k > 0 && k < n) cut = radix_cut<false>(x, n, w, cut, (u64)k, hist, share);
-    const float p = a.top_p ? a.top_p[row] : 1.f;
-    if (p < 1.f) {
-        // the sum of what top-k keeps
-        if (tid == 0) share[0] = 0;
+    Cut cut{0u, kMaxVocab};
+    if (info.cut == 1) {
+        const u64* src = row_list(a, row);
+        for (int i = tid; i < count; i += kRowThreads) list[i] = src[i];
         __syncthreads();
-        u64 mine = 0;
-        for (int i = tid; i < n; i += kThreads)
-            if (order_key(x[i]) > cut.key) mine += (u64)(w(x[i]) * kUnit + 0.5);
-        atomicAdd(&share[0], mine);
-        __syncthreads();
-        u64 total = share[0];
-        if (cut.key > 0) {
-            const float l =
-                __uint_as_float((cut.key & 0x80000000u) ? cut.key ^ 0x80000000u : ~cut.key);
-            total += (u64)cut.ties * (u64)(w(l) * kUnit + 0.5);
+        const float base = bin_of(l_max, s.per_l);
+        auto each = [&](auto f) {
+            for (int i = tid; i < count; i += kRowThreads)
+                f((uint32_t)(list[i] >> 32), (int)(uint32_t)list[i]);
+        };
+        auto bin = [&](uint32_t key) { return bin_below(base, bin_of(key_logit(key), s.per_l)); };
+        u64 kept_w = info.w_all;
+        if (info.use_k) {
+            auto in_k = [&](auto f) {
+                each([&](uint32_t key, int i) {
+                    if (bin(key) == info.k_bin) f(key, i);
+                });
+            };
+            cut = select_cut(sel, (u64)(s.k - info.k_before), in_k, one);
+            if (s.use_p) {
+                u64 add = 0;
+                in_k([&](uint32_t key, int i) { add += cut.keeps(key, i) ? units(key) : 0; });
+                if (add) atomicAdd(&total_w, add);
+                __syncthreads();
+                kept_w = info.w_before_k + total_w;
+            }
         }
-        __syncthreads();
-        u64 target = p > 0.f ? (u64)ceil((double)p * (double)total) : 1;
-        target = target < 1 ? 1 : target > total ? total : target;
-        cut = radix_cut<true>(x, n, w, cut, target, hist, share);
-    }
-    const float mp = a.min_p ? a.min_p[row] : 0.f;
-    const double min_w = mp > 0.f ? fmin((double)mp, 1.0) : 0.0;  // NaN: off
-
-    // A wave takes a run of indices; its kept ties, then its kept sum.
-    const int run = ((n + kWaves - 1) / kWaves + 63) / 64 * 64;
-    const int i0 = min(wave * run, n), i1 = min(i0 + run, n);
-    int ties = 0;
-    for (int i = i0 + lane; i < i1; i += 64) ties += order_key(x[i]) == cut.key;
-    for (int off = 32; off; off >>= 1) ties += __shfl_xor(ties, off, 64);
-    __syncthreads();
-    if (lane == 0) wave_n[wave] = ties;
-    __syncthreads();
-    int before = 0;
-    for (int i = 0; i < wave; i++) before += wave_n[i];
-    // walks the run 64 indices at a time: f(i, kept weight of the lane)
-    auto walk = [&](auto f) {
-        int seen = before;
-        for (int b = i0; b < i1; b += 64) {
-            const int i = b + lane;
-            const float l = i < i1 ? x[i] : -INFINITY;
-            const uint32_t key = order_key(l);
-            const u64 tie = __ballot(i < i1 && key == cut.key);
-            const int rank = seen + __popcll(tie & ((1ull << lane) - 1));
-            seen += __popcll(tie);
-            double v = 0.0;
-            if (i < i1 && (key > cut.key || (key == cut.key && rank < cut.ties))) {
-                v = w(l);
-                if (!(v >= min_w)) v = 0.0;
-            }
-            if (f(i, v)) return;
+        if (s.use_p) {
+            const u64 goal = p_goal(s, kept_w);
+            const Cut k_cut = cut;
+            cut = select_cut(
+                sel, goal > info.w_before_lo ? goal - info.w_before_lo : 1,
+                [&](auto f) {
+                    each([&](uint32_t key, int i) {
+                        const int b = bin(key);
+                        if (b >= info.lo && b <= info.hi && k_cut.keeps(key, i)) f(key, i);
+                    });
+                },
+                units);
+            cut.within(k_cut);
         }
-    };
-    double sum = 0.0;
-    walk([&](int, double v) {
-        sum += v;
-        return false;
-    });
-    sum = wave_sum(sum);
-    if (lane == 0) wave_w[wave] = sum;
-    __syncthreads();
-    double total = 0.0, ahead = 0.0;
-    int last = 0;
-    for (int i = 0; i < kWaves; i++) {
-        if (i < wave) ahead += wave_w[i];
-        total += wave_w[i];
-        if (wave_w[i] > 0.0) last = i;
-    }
-    double u = a.u ? (double)a.u[row] : 0.0;
-    u = u > 0.0 ? u : 0.0;  // NaN: 0
-    const double target = u * total;
-    // the wave in whose run the sum passes the target, or the last one that has any
-    const bool here = (ahead <= target && ahead + sum > target) || (wave == last && target >= total);
-    if (here) {
-        double at = ahead;
-        int best = -1;
-        walk([&](int i, double v) {
-            double c = v;
-            for (int off = 1; off < 64; off <<= 1) {
-                const double o = __shfl_up(c, off, 64);
-                if (lane >= off) c += o;
-            }
-            c += at;
-            const u64 over = __ballot(v > 0.0 && c > target);
-            const u64 any = __ballot(v > 0.0);
-            if (over) {
-                best = i - lane + __builtin_ctzll(over);
-                return true;
-            }
-            if (any) best = i - lane + 63 - __builtin_clzll(any);
-            at = __shfl(c, 63, 64);
-            return false;
+        // what the list adds to each chunk
+        each([&](uint32_t key, int i) {
+            if (!cut.keeps(key, i)) return;
+            const double we = w(key_logit(key));
+            if (we >= s.min_w) atomicAdd(&chunk_add[i / a.chunk], row_units(we));
         });
-        if (lane == 0 && best >= 0) atomicMax(&answer, best);
+        __syncthreads();
+    } else if (info.cut == 2) {
+        auto each = [&](auto f) {
+            for (int i = tid; i < n; i += kRowThreads) {
+                const uint32_t key = order_key(x[i]);
+                if (key > kKeyMinusInf) f(key, i);
+            }
+        };
+        if (s.use_k) cut = select_cut(sel, (u64)s.k, each, one);
+        if (s.use_p) {
+            u64 add = 0;
+            const Cut k_cut = cut;
+            auto kept = [&](auto f) {
+                each([&](uint32_t key, int i) {
+                    if (k_cut.keeps(key, i)) f(key, i);
+                });
+            };
+            kept([&](uint32_t key, int) { add += units(key); });
+            if (add) atomicAdd(&total_w, add);
+            __syncthreads();
+            cut = select_cut(sel, p_goal(s, total_w), kept, units);
+            cut.within(k_cut);
+        }
     }
-    __syncthreads();
-    if (tid == 0) a.out[row] = answer >= 0 ? answer : first_max;
+
+    // ---- the running sum over chunks, then inside the one that passes u times the sum
+    auto weight_at = [&](int i) {
+        const float l = x[i];
+        if (!cut.keeps(order_key(l), i)) return 0.0;
+        const double v = w(l);
+        return v >= s.min_w ? v : 0.0;
+    };
+    int c0 = 0, c1 = n;  // the range to walk
+    double before = 0.0, total = 0.0;
+    double u = (double)a.u[row];
+    u = u > 0.0 ? u : 0.0;  // NaN: 0
+    const bool by_chunk = s.plain() ? !w.inf : info.cut != 2 && !w.inf;
+    if (by_chunk) {
+        // every wave scans the (at most 64) chunks for itself
+        double v = 0.0;
+        if (lane < a.chunks && mine_c.top > -INFINITY)
+            v = s.plain() ? mine_c.sum * w(mine_c.top)
+                          : mine_c.sum + (double)chunk_add[lane] * (1.0 / kRowUnit);
+        double upto = v;
+        for (int off = 1; off < 64; off <<= 1) {
+            const double o = __shfl_up(upto, off, 64);
+            if (lane >= off) upto += o;
+        }
+        total = __shfl(upto, 63, 64);
+        const u64 pass = __ballot(v > 0.0 && upto > u * total), any = __ballot(v > 0.0);
+        const int who = pass ? __builtin_ctzll(pass) : any ? 63 - __builtin_clzll(any) : 0;
+        before = __shfl(upto, who, 64) - __shfl(v, who, 64);
+        c0 = who * a.chunk;
+        c1 = min(c0 + a.chunk, n);
+    } else {
+        double sum = 0.0;
+        for (int i = tid; i < n; i += kRowThreads) sum += weight_at(i);
+        sum = wave_sum(sum);
+        if (lane == 0) wave_w[wave] = sum;
+        __syncthreads();
+        for (int i = 0; i < kRowWaves; i++) total += wave_w[i];
+        __syncthreads();
+    }
+    const double target = u * total;
+    constexpr int kEach = 8;
+    for (int b = c0; b < c1; b += kRowThreads * kEach) {  // kEach indices in a row a thread
+        double v[kEach], sum = 0.0;
+        int last = -1;
+#pragma unroll
+        for (int e = 0; e < kEach; e++) {
+            const int i = b + kEach * tid + e;
+            v[e] = i < c1 ? weight_at(i) : 0.0;
+            sum += v[e];
+            if (v[e] > 0.0) last = i;
+        }
+        double upto = sum;
+        for (int off = 1; off < 64; off <<= 1) {
+            const double o = __shfl_up(upto, off, 64);
+            if (lane >= off) upto += o;
+        }
+        if (lane == 63) wave_w[wave] = upto;
+        __syncthreads();
+        double all = 0.0, ahead = before;
+        for (int i = 0; i < kRowWaves; i++) {
+            if (i < wave) ahead += wave_w[i];
+            all += wave_w[i];
+        }
+        double run = ahead + upto - sum;
+        int hit = -1;
+#pragma unroll
+        for (int e = 0; e < kEach; e++) {
+            run += v[e];
+            if (hit < 0 && v[e] > 0.0 && run > target) hit = b + kEach * tid + e;
+        }
+        // the first index that passes; where rounding leaves none, the last kept one
+        const u64 hits = __ballot(hit >= 0);
+        if (tid == 0) answer = -1, total_w = ~0ull;
+        __syncthreads();
+        if (hits && lane == __builtin_ctzll(hits)) atomicMin(&total_w, (u64)hit);
+        if (last >= 0) atomicMax(&answer, last);
+        __syncthreads();
+        const u64 found = total_w;
+        const int kept = answer;
+        before += all;
+        if (found != ~0ull) {
+            if (tid == 0) a.out[row] = (int)found;
+            return;
+        }
+        if (kept >= 0 && tid == 0) a.out[row] = kept;
+        __syncthreads();
+    }
+}
+
+int chunk_of(int n_rows, int n_vocab) {
+    // Chunks of 8192 elements, the workgroup's registers; longer ones where the rows
+    // alone give every CU two, as each of them adds up the histograms of all.
+    int chunk = kBlock;
+    while (chunk < 16 * kBlock && (long long)n_rows * ((n_vocab + 2 * chunk - 1) / (2 * chunk)) >= 512)
+        chunk *= 2;
+    return chunk;
+}
+
+long long row_bytes_of(int chunks) {
+    return 128 + 8LL * kList + (long long)chunks * (sizeof(ChunkStat) + kBins * 12);
 }
 
 }  // namespace
 
 extern "C" long long tf_sample_ws_bytes(int n_rows, int n_vocab) {
-    return n_rows > 0 && n_vocab > 0 && n_vocab < (1 << 19) ? 256LL * n_rows : -1;
+    if (n_rows <= 0 || n_vocab <= 0 || n_vocab >= kMaxVocab) return -1;
+    const int chunk = chunk_of(n_rows, n_vocab);
+    return n_rows * row_bytes_of((n_vocab + chunk - 1) / chunk);
 }
 
 extern "C" int tf_sample(const float* logits, int n_rows, int n_vocab, int row_stride,
@@ -271,9 +799,27 @@ extern "C" int tf_sample(const float* logits, int n_rows, int n_vocab, int row_s
                          const float* min_p, const float* u, int* out_idx, void* ws,
                          long long ws_bytes, tf_stream_t stream) {
     TF_CHECK_ARG(logits && u && out_idx && ws && n_rows > 0 && n_vocab > 0);
-    TF_CHECK_ARG(n_vocab < (1 << 19) && row_stride >= n_vocab);
-    TF_CHECK_ARG(ws_bytes >= tf_sample_ws_bytes(n_rows, n_vocab) && ((uintptr_t)ws & 15) == 0);
-    const SampleArgs a{logits, row_stride, n_vocab, temperature, top_k, top_p, min_p, u, out_idx};
-    hipLaunchKernelGGL(tf_sample_row_kernel, dim3(n_rows), dim3(kThreads), 0, tf_stream(stream), a);
+    TF_CHECK_ARG(n_vocab < kMaxVocab && row_stride >= n_vocab && ((uintptr_t)ws & 15) == 0);
+    TF_CHECK_ARG(ws_bytes >= tf_sample_ws_bytes(n_rows, n_vocab));
+    SampleArgs a{};
+    a.logits = logits, a.stride = row_stride, a.n = n_vocab;
+    a.temperature = temperature, a.top_k = top_k, a.top_p = top_p, a.min_p = min_p;
+    a.u = u, a.out = out_idx;
+    a.chunk = chunk_of(n_rows, n_vocab);
+    a.chunks = (n_vocab + a.chunk - 1) / a.chunk;
+    a.ws = static_cast<uint8_t*>(ws);
+    a.row_bytes = row_bytes_of(a.chunks);
+    TF_CHECK_ARG((long long)n_rows * a.chunks <= (long long)(UINT32_MAX / kRowThreads));
+    const unsigned grid = (unsigned)n_rows * (unsigned)a.chunks;
+    hipLaunchKernelGGL(tf_sample_stats_kernel, dim3(grid), dim3(kChunkThreads), 0,
+                       tf_stream(stream), a);
+    if (top_k || top_p || min_p)
+        hipLaunchKernelGGL(tf_sample_gather_kernel, dim3(grid), dim3(kChunkThreads), 0,
+                           tf_stream(stream), a);
+    constexpr int bytes = 8 * (kList + kMaxChunks) + (int)sizeof(Select);
+    const int rc = tf_set_lds_limit((const void*)tf_sample_draw_kernel, bytes);
+    if (rc) return rc;
+    hipLaunchKernelGGL(tf_sample_draw_kernel, dim3(n_rows), dim3(kRowThreads), bytes,
+                       tf_stream(stream), a);
     return TF_LAUNCH_RESULT();
 }
