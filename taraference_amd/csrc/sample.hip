@@ -20,7 +20,7 @@
 // named by its last element, and no row is sorted.  Three launches, rows cut
 // into chunks so that one row has the loads of many CUs:
 //   1. stats: a chunk's largest logit, and a histogram of counts and weights
-//      over bins of 1/16 of z below it (no filter: its sum of weights);
+//      over bins of 1/8 of z below it (no filter: its sum of weights);
 //   2. gather: each chunk's workgroup adds the row's histograms, finds the bins
 //      in which the cuts of top-k and top-p lie, writes its elements of those
 //      bins to the row's list, and adds up the weights of the bins before them;
@@ -41,13 +41,16 @@ namespace {
 
 typedef unsigned long long u64;
 
-constexpr int kBins = 512;          // of 1/16 of z: 32 below a chunk's largest, the last open
-constexpr float kPerZ = 16.f;
-constexpr int kList = 8192;         // elements of a row's list
+constexpr int kBins = 256;          // of 1/8 of z: 32 below a chunk's largest, the last open
+constexpr float kPerZ = 8.f;
+constexpr int kList = 8192;         // elements of a row's list, and
+constexpr int kChunkList = 2048;    // of a chunk's part of it
 constexpr int kChunkThreads = 512, kChunkWaves = kChunkThreads / 64;
 constexpr int kBlock = 16 * kChunkThreads;  // elements that a chunk's workgroup holds at once
 constexpr int kMaxVocab = 1 << 19;
 constexpr int kMaxChunks = kMaxVocab / kBlock;  // 64
+constexpr int kSegment = 1024;                  // elements of a wave: what the draw walks
+constexpr int kMaxSegments = kMaxVocab / kSegment;
 constexpr int kRowThreads = 1024, kRowWaves = kRowThreads / 64;
 // Integer weights: a chunk has at most 2^17 elements, a row fewer than 2^19, so that
 // their sums stay below 2^63.
@@ -91,27 +94,31 @@ struct RowInfo {
 struct ChunkStat {
     float top;    // the largest logit
     int index;    // its lowest index (T <= 0 only)
-    double sum;   // weights: of the chunk (no filter; of its largest), or kept for sure (of the row's)
+    int listed;   // elements of its list
+    int pad;
 };
 __device__ __forceinline__ RowInfo* row_info(const SampleArgs& a, int row) {
     return reinterpret_cast<RowInfo*>(a.ws + row * a.row_bytes);
 }
-__device__ __forceinline__ int* row_count(const SampleArgs& a, int row) {
-    return reinterpret_cast<int*>(a.ws + row * a.row_bytes + 120);
-}
-__device__ __forceinline__ u64* row_list(const SampleArgs& a, int row) {
-    return reinterpret_cast<u64*>(a.ws + row * a.row_bytes + 128);
-}
 __device__ __forceinline__ ChunkStat* row_stats(const SampleArgs& a, int row) {
-    return reinterpret_cast<ChunkStat*>(row_list(a, row) + kList);
+    return reinterpret_cast<ChunkStat*>(a.ws + row * a.row_bytes + 128);
+}
+// Of each segment: the sum of its weights, of its chunk's largest (no filter; f64), or
+// of the row's, of what is kept for sure (kRowUnit).
+__device__ __forceinline__ u64* segment_sums(const SampleArgs& a, int row) {
+    return reinterpret_cast<u64*>(row_stats(a, row) + kMaxChunks);
+}
+constexpr int kChunkWords = kChunkList + kBins + kBins / 2;
+__device__ __forceinline__ u64* chunk_list(const SampleArgs& a, int row, int c) {
+    return segment_sums(a, row) + kMaxSegments + (size_t)c * kChunkWords;
 }
 __device__ __forceinline__ u64* chunk_weights(const SampleArgs& a, int row, int c) {
-    return reinterpret_cast<u64*>(row_stats(a, row) + a.chunks) + (size_t)c * (kBins + kBins / 2);
+    return chunk_list(a, row, c) + kChunkList;
 }
 __device__ __forceinline__ uint32_t* chunk_counts(const SampleArgs& a, int row, int c) {
     return reinterpret_cast<uint32_t*>(chunk_weights(a, row, c) + kBins);
 }
-static_assert(sizeof(RowInfo) <= 120, "the list's count follows");
+static_assert(sizeof(RowInfo) <= 128 && sizeof(ChunkStat) == 16, "the workspace's layout");
 
 struct Settings {
     float temp;
@@ -124,22 +131,25 @@ struct Settings {
     __device__ bool plain() const { return !use_k && !use_p && !(min_w > 0.0); }
 };
 __device__ __forceinline__ Settings settings(const SampleArgs& a, int row) {
+    // one value a workgroup: kept scalar, so that branches on them are
+    auto uni = [](float v) { return tf_readlane(v, 0); };
     Settings s;
-    s.temp = a.temperature ? a.temperature[row] : 1.f;
+    s.temp = uni(a.temperature ? a.temperature[row] : 1.f);
     s.greedy = !(s.temp > 0.f);
-    s.k = a.top_k ? a.top_k[row] : 0;
+    s.k = __builtin_amdgcn_readfirstlane(a.top_k ? a.top_k[row] : 0);
     s.use_k = s.k > 0 && s.k < a.n;
-    s.p = a.top_p ? a.top_p[row] : 1.f;
+    s.p = uni(a.top_p ? a.top_p[row] : 1.f);
     s.use_p = s.p < 1.f;
-    const float m = a.min_p ? a.min_p[row] : 0.f;
+    const float m = uni(a.min_p ? a.min_p[row] : 0.f);
     s.min_w = m > 0.f ? fmin((double)m, 1.0) : 0.0;
-    s.per_l = kPerZ / s.temp;
+    s.per_l = uni(kPerZ / s.temp);
     s.bad = !(s.temp >= 1e-6f);
     return s;
 }
-// Whether the bins can hold a row with this largest logit.
+// Whether the bins can hold a row with this largest logit: their numbers are exact
+// floats up to 2^23.
 __device__ __forceinline__ bool no_bins(const Settings& s, float l_max) {
-    return s.bad || !(fabsf(l_max) * s.per_l < 1e9f);
+    return s.bad || !(fabsf(l_max) * s.per_l < 0x1p22f);
 }
 // The bin of a logit, counted from that of `base`; both by the same monotone product.
 __device__ __forceinline__ float bin_of(float l, float per_l) { return floorf(l * per_l); }
@@ -215,16 +225,56 @@ __device__ __forceinline__ u64 row_units(double w) {
     return __builtin_bit_cast(u64, w + 256.0) - __builtin_bit_cast(u64, 256.0);
 }
 
-__device__ __forceinline__ double wave_sum(double v) {
-    for (int off = 32; off; off >>= 1) v += __shfl_xor(v, off, 64);
+// Inclusive sum over the wave's lanes, in DPP row shifts and broadcasts: a tenth of
+// the latency of six exchanges through LDS.
+template <int CTRL, int ROWS, class T>
+__device__ __forceinline__ T dpp_or_0(T v) {
+    if constexpr (sizeof(T) == 4) {
+        return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL,
+                                                                 ROWS, 0xF, false));
+    } else {
+        const u64 b = __builtin_bit_cast(u64, v);
+        const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, ROWS, 0xF, false);
+        const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(b >> 32), CTRL, ROWS, 0xF, false);
+        return __builtin_bit_cast(T, (u64)hi << 32 | lo);
+    }
+}
+template <class T>
+__device__ __forceinline__ T wave_scan(T v) {
+    v += dpp_or_0<0x111, 0xF>(v);  // row_shr 1, 2, 4, 8
+    v += dpp_or_0<0x112, 0xF>(v);
+    v += dpp_or_0<0x114, 0xF>(v);
+    v += dpp_or_0<0x118, 0xF>(v);
+    v += dpp_or_0<0x142, 0xA>(v);  // lane 15 of a row to the next row, of rows 1 and 3
+    v += dpp_or_0<0x143, 0xC>(v);  // lane 31 to rows 2 and 3
     return v;
 }
+template <class T>
+__device__ __forceinline__ T lane_value(T v, int lane) {
+    if constexpr (sizeof(T) == 4) {
+        return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
+    } else {
+        const u64 b = __builtin_bit_cast(u64, v);
+        const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)b, lane);
+        const uint32_t hi = __builtin_amdgcn_readlane((int)(b >> 32), lane);
+        return __builtin_bit_cast(T, (u64)hi << 32 | lo);
+    }
+}
+template <class T>
+__device__ __forceinline__ T wave_sum(T v) {
+    return lane_value(wave_scan(v), 63);
+}
 
-// Elements i0 + 4 * tid + 2048 j + 0 .. 3 of a row; past `end`: -inf.
+// A block's elements: a wave holds a segment, a lane index(e) = i0 + 1024 wave + 256 (e
+// / 4) + 4 lane + e % 4; past `end`: -inf.
+__device__ __forceinline__ int block_index(int i0, int e) {
+    return i0 + kSegment * (int)(threadIdx.x >> 6) + 256 * (e >> 2) + 4 * (int)(threadIdx.x & 63) +
+           (e & 3);
+}
 __device__ __forceinline__ void load_block(const float* x, int i0, int end, float (&v)[16]) {
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-        const int i = i0 + 4 * (int)threadIdx.x + 4 * kChunkThreads * j;
+        const int i = block_index(i0, 4 * j);
         if (i + 3 < end) {
             const tf_u32x4 b = tf_ld16_a4(x + i);
 #pragma unroll
@@ -235,14 +285,28 @@ __device__ __forceinline__ void load_block(const float* x, int i0, int end, floa
         }
     }
 }
-__device__ __forceinline__ int block_index(int i0, int e) {
-    return i0 + 4 * (int)threadIdx.x + 4 * kChunkThreads * (e >> 2) + (e & 3);
+
+// Four elements at a time, the others moved down behind them: f(j, v[0 .. 3]) for
+// elements 4 j ..  A quarter of the code of sixteen in a row, and the time of a cold
+// instruction cache with it.
+template <class F>
+__device__ __forceinline__ void each_four(float (&v)[16], F f) {
+#pragma unroll 1
+    for (int j = 0; j < 4; j++) {
+        f(j);
+        const float a[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+        for (int i = 0; i < 12; i++) v[i] = v[i + 4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[12 + i] = a[i];
+    }
 }
 
-__global__ __launch_bounds__(kChunkThreads) void tf_sample_stats_kernel(SampleArgs a) {
-    __shared__ u64 weight[kBins];
-    __shared__ uint32_t count[kBins];
-    __shared__ double table[32], dpart[kChunkWaves];
+__global__ __launch_bounds__(kChunkThreads, 6) void tf_sample_stats_kernel(SampleArgs a) {
+    // four of each bin, by lane: half of a wave's elements may share one
+    __shared__ u64 weight[kBins][4];
+    __shared__ uint32_t count[kBins][4];
+    __shared__ double table[32];
     __shared__ float part[kChunkWaves];
     __shared__ int first;
     const int row = blockIdx.x / a.chunks, c = blockIdx.x - row * a.chunks;
@@ -254,7 +318,7 @@ __global__ __launch_bounds__(kChunkThreads) void tf_sample_stats_kernel(SampleAr
     load_block(x, i0, end, v);
     const Settings s = settings(a, row);
     fill_exp2(table);
-    for (int i = tid; i < kBins; i += kChunkThreads) weight[i] = 0, count[i] = 0;
+    for (int i = tid; i < 4 * kBins; i += kChunkThreads) weight[0][i] = 0, count[0][i] = 0;
     if (tid == 0) first = a.n;
     float top = -INFINITY;  // fmaxf passes NaN by
 #pragma unroll
@@ -269,7 +333,6 @@ __global__ __launch_bounds__(kChunkThreads) void tf_sample_stats_kernel(SampleAr
     __syncthreads();
     for (int i = 0; i < kChunkWaves; i++) top = fmaxf(top, part[i]);
     ChunkStat* stat = row_stats(a, row) + c;
-    if (c == 0 && tid == 0) *row_count(a, row) = 0;
     if (tid == 0) stat->top = top;
     const bool empty = !(top > -INFINITY);
     if (s.greedy) {
@@ -285,18 +348,18 @@ __global__ __launch_bounds__(kChunkThreads) void tf_sample_stats_kernel(SampleAr
     if (!s.filtered() && !s.plain()) return;
     const RowWeight w(table, s.temp, top);
     if (s.plain()) {
-        double sum = 0.0;
-        for (int b = i0; b < end && !empty; b += kBlock) {
+        for (int b = i0; b < end; b += kBlock) {
             if (many) load_block(x, b, end, v);
+            double sum = 0.0;
+            if (!empty)
+                each_four(v, [&](int) {
 #pragma unroll
-            for (int e = 0; e < 16; e++) sum += w(v[e]);
-        }
-        sum = wave_sum(sum);
-        if (lane == 0) dpart[wave] = sum;
-        __syncthreads();
-        if (tid == 0) {
-            for (int i = 1; i < kChunkWaves; i++) sum += dpart[i];
-            stat->sum = sum;
+                    for (int e = 0; e < 4; e++) sum += w(v[e]);
+                });
+            sum = wave_sum(sum);
+            const int seg = (b >> 10) + wave;
+            if (lane == 0 && seg * kSegment < a.n)
+                segment_sums(a, row)[seg] = __builtin_bit_cast(u64, sum);
         }
         return;
     }
@@ -304,42 +367,34 @@ __global__ __launch_bounds__(kChunkThreads) void tf_sample_stats_kernel(SampleAr
         const float base = bin_of(top, s.per_l);
         for (int b = i0; b < end; b += kBlock) {
             if (many) load_block(x, b, end, v);
+            each_four(v, [&](int) {
 #pragma unroll
-            for (int e = 0; e < 16; e++) {
-                if (!(v[e] > -INFINITY)) continue;  // NaN too
-                const int bin = bin_below(base, bin_of(v[e], s.per_l));
-                atomicAdd(&count[bin], 1u);
-                if (s.use_p) atomicAdd(&weight[bin], chunk_units(w(v[e])));
-            }
+                for (int e = 0; e < 4; e++) {  // -inf and NaN add nothing
+                    const int bin = bin_below(base, bin_of(v[e], s.per_l));
+                    if (s.use_k) atomicAdd(&count[bin][lane & 3], v[e] > -INFINITY ? 1u : 0u);
+                    if (s.use_p) atomicAdd(&weight[bin][lane & 3], chunk_units(w(v[e])));
+                }
+            });
         }
     }
     __syncthreads();
     u64* gw = chunk_weights(a, row, c);
     uint32_t* gc = chunk_counts(a, row, c);
-    for (int i = tid; i < kBins; i += kChunkThreads) gw[i] = weight[i], gc[i] = count[i];
-}
-
-// Inclusive scan over the workgroup (kChunkThreads threads), in thread order.
-template <class T>
-__device__ __forceinline__ T block_scan(T v, T* part /* kChunkWaves, LDS */) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int off = 1; off < 64; off <<= 1) {
-        const T o = __shfl_up(v, off, 64);
-        if (lane >= off) v += o;
+    // the first half of the workgroup writes counts, the second weights
+    const int bin = tid % kBins;
+    if (tid < kBins) {
+        if (s.use_k) gc[bin] = count[bin][0] + count[bin][1] + count[bin][2] + count[bin][3];
+    } else if (s.use_p) {
+        gw[bin] = weight[bin][0] + weight[bin][1] + weight[bin][2] + weight[bin][3];
     }
-    if (lane == 63) part[wave] = v;
-    __syncthreads();
-    T before = 0;
-    for (int i = 0; i < wave; i++) before += part[i];
-    __syncthreads();
-    return v + before;
 }
 
-__global__ __launch_bounds__(kChunkThreads) void tf_sample_gather_kernel(SampleArgs a) {
-    __shared__ u64 w_upto[kBins], wpart[kChunkWaves];
-    __shared__ int n_upto[kBins], ipart[kChunkWaves];
-    __shared__ double table[32], dpart[kChunkWaves], chunk_f[kMaxChunks];
-    __shared__ int chunk_shift[kMaxChunks], first[3], share;
+static_assert(kChunkThreads == 2 * kBins, "a half for counts, a half for weights");
+__global__ __launch_bounds__(kChunkThreads, 6) void tf_sample_gather_kernel(SampleArgs a) {
+    __shared__ u64 n_upto[kBins], w_upto[kBins], part[kChunkWaves];  // totals up to a bin
+    __shared__ double table[32], chunk_f[kMaxChunks];
+    __shared__ float kept[kChunkWaves][kSegment];
+    __shared__ int chunk_shift[kMaxChunks], first[3], place;
     const int row = blockIdx.x / a.chunks, c = blockIdx.x - row * a.chunks;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const float* x = a.logits + (size_t)row * a.stride;
@@ -350,6 +405,8 @@ __global__ __launch_bounds__(kChunkThreads) void tf_sample_gather_kernel(SampleA
     const Settings s = settings(a, row);
     float mine_top = -INFINITY;
     if (lane < a.chunks) mine_top = row_stats(a, row)[lane].top;
+    // the workgroup's first half adds up the histograms' counts, the second their weights
+    const int half = tid / kBins, bin = tid % kBins;
     fill_exp2(table);
     if (s.greedy || s.plain()) return;
     const float l_max = tf_wave_max(mine_top);
@@ -361,64 +418,66 @@ __global__ __launch_bounds__(kChunkThreads) void tf_sample_gather_kernel(SampleA
         return;
     }
     const float base = bin_of(l_max, s.per_l);
-    w_upto[tid] = 0;
-    n_upto[tid] = 0;
+    u64* upto_of = half ? w_upto : n_upto;
+    upto_of[bin] = 0;
     if (tid < 3) first[tid] = kBins - 1;
+    if (tid == 0) place = 0;
     __syncthreads();  // the table
     const RowWeight w(table, s.temp, l_max);
     int lo = kBins, hi = -1, k_bin = -1;  // min-p alone: every bin is kept for sure
     if (s.filtered()) {
         // bin b of the row: the chunks' bins, shifted by how far their largest lies below
         // the row's, and their weights scaled alike; what falls past the last bin goes
-        // there.  Eight chunks' loads at once: one after the other they were half the time.
+        // there
         if (wave == 0) {
             const bool any = mine_top > -INFINITY;
             chunk_f[lane] = any ? w(mine_top) * (kRowUnit / kChunkUnit) : 0.0;
             chunk_shift[lane] = any ? bin_below(base, bin_of(mine_top, s.per_l)) : 0;
         }
         __syncthreads();
-        for (int c8 = 0; c8 < a.chunks; c8 += 8) {
-            uint32_t nc[8];
-            u64 nw[8];
+        if (half ? s.use_p : s.use_k)
+            for (int c0 = 0; c0 < a.chunks; c0 += 8) {
+                u64 got[8];
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const int cc = min(c8 + i, a.chunks - 1);
-                nc[i] = chunk_counts(a, row, cc)[tid];
-                nw[i] = s.use_p ? chunk_weights(a, row, cc)[tid] : 0;
-            }
+                for (int i = 0; i < 8; i++) {
+                    const int cc = min(c0 + i, a.chunks - 1);
+                    got[i] = half ? chunk_weights(a, row, cc)[bin] : chunk_counts(a, row, cc)[bin];
+                }
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                if (c8 + i >= a.chunks || nc[i] == 0) continue;
-                const int b = min(tid + chunk_shift[c8 + i], kBins - 1);
-                atomicAdd(&n_upto[b], (int)nc[i]);
-                if (s.use_p) atomicAdd(&w_upto[b], (u64)((double)nw[i] * chunk_f[c8 + i] + 0.5));
+                for (int i = 0; i < 8; i++) {
+                    if (c0 + i >= a.chunks || got[i] == 0) continue;
+                    if (half) got[i] = (u64)((double)got[i] * chunk_f[c0 + i] + 0.5);
+                    atomicAdd(&upto_of[min(bin + chunk_shift[c0 + i], kBins - 1)], got[i]);
+                }
             }
-        }
         __syncthreads();
-        const u64 wt = block_scan(w_upto[tid], wpart);
-        const int nt = block_scan(n_upto[tid], ipart);
-        w_upto[tid] = wt;
-        n_upto[tid] = nt;
+        u64 upto = wave_scan(upto_of[bin]);
+        if (lane == 63) part[wave] = upto;
         __syncthreads();
-        const bool use_k = s.use_k && n_upto[kBins - 1] > s.k;
-        if (use_k && nt >= s.k && (tid == 0 || n_upto[tid - 1] < s.k)) first[0] = tid;
+        for (int i = half * (kChunkWaves / 2); i < wave; i++) upto += part[i];
+        upto_of[bin] = upto;
+        __syncthreads();
+        // the bin in which a running total reaches a goal; one thread's
+        auto reach = [&](u64 goal, int slot) {
+            if (upto >= goal && (bin == 0 || upto_of[bin - 1] < goal)) first[slot] = bin;
+        };
+        const bool use_k = s.use_k && n_upto[kBins - 1] > (u64)s.k;
+        if (use_k && !half) reach((u64)s.k, 0);
         __syncthreads();
         info.use_k = use_k;
         if (use_k) {
             k_bin = first[0];
-            info.k_before = k_bin ? n_upto[k_bin - 1] : 0;
+            info.k_before = k_bin ? (int)n_upto[k_bin - 1] : 0;
             info.w_before_k = k_bin ? w_upto[k_bin - 1] : 0;
             lo = hi = k_bin;
         }
         info.w_all = w_upto[kBins - 1];
         if (s.use_p) {
             // the goal is p of what top-k keeps: between these two until k_bin is resolved
-            auto reach = [&](u64 all, int slot) {
-                const u64 goal = p_goal(s, all);
-                if (wt >= goal && (tid == 0 || w_upto[tid - 1] < goal)) first[slot] = tid;
-            };
-            reach(use_k ? info.w_before_k : info.w_all, 1);
-            reach(use_k ? w_upto[k_bin] : info.w_all, 2);
+            if (half) {
+                reach(p_goal(s, use_k ? info.w_before_k : info.w_all), 1);
+                reach(p_goal(s, use_k ? w_upto[k_bin] : info.w_all), 2);
+            }
             __syncthreads();
             lo = first[1];
             hi = first[2];
@@ -430,10 +489,12 @@ __global__ __launch_bounds__(kChunkThreads) void tf_sample_gather_kernel(SampleA
             info.cut = 1;
             info.w_before_lo = lo ? w_upto[lo - 1] : 0;
             auto in_bins = [&](int b0, int b1) { return n_upto[b1] - (b0 ? n_upto[b0 - 1] : 0); };
-            const int listed = in_bins(lo, hi) + (k_bin > hi ? in_bins(k_bin, k_bin) : 0);
+            // with top-k the list's length is known here; else the draw finds it too long
+            const u64 listed = in_bins(lo, hi) + (k_bin > hi ? in_bins(k_bin, k_bin) : 0);
             // min-p above the first listed bin (by a bin and the rounding of the bins'
             // products): the cuts are past it
-            if (fabsf(base) < 1e5f && s.min_w > exp((2 - lo) * (1.0 / kPerZ))) {
+            if (fabsf(base) < 1e5f && lo > 2 &&
+                s.min_w > exp2_neg((2 - lo) * (1.44269504088896340736 / kPerZ), table)) {
                 info.cut = 0;
                 lo = kBins, hi = -1, k_bin = -1;
             } else if (listed > kList) {
@@ -445,42 +506,52 @@ __global__ __launch_bounds__(kChunkThreads) void tf_sample_gather_kernel(SampleA
     if (c == 0 && tid == 0) *row_info(a, row) = info;
     if (info.cut == 2) return;
     // the chunk's weight before bin lo, and its part of the list
-    double sum = 0.0;
+    // bins as bounds on the product that bin_of() rounds down: bin b holds base - b <= l
+    // per_l < base - b + 1, the last one all below
+    const float sure = lo < kBins ? base - (float)(lo - 1) : -INFINITY;
+    const float listed = hi < kBins - 1 ? base - (float)hi : -INFINITY;
+    const float k_from = k_bin < 0 ? INFINITY : k_bin < kBins - 1 ? base - (float)k_bin : -INFINITY;
+    const float k_to = base - (float)(k_bin - 1);
     for (int b = i0; b < end; b += kBlock) {
         if (many) load_block(x, b, end, v);
-        uint32_t mine = 0;
+        // the segment's elements that are kept for sure, side by side in LDS: few of a
+        // lane's are, and a branch for each would form weights in every wave
+        int n_kept = 0;
+        each_four(v, [&](int j) {
 #pragma unroll
-        for (int e = 0; e < 16; e++) {
-            if (!(v[e] > -INFINITY)) continue;
-            const int bin = bin_below(base, bin_of(v[e], s.per_l));
-            if (bin < lo) {
-                const double we = w(v[e]);
-                sum += we >= s.min_w ? we : 0.0;
-            } else if (bin <= hi || bin == k_bin) {
-                mine |= 1u << e;
+            for (int e = 0; e < 4; e++) {
+                const float m = v[e] * s.per_l;
+                const bool is = v[e] > -INFINITY, in = is && (m >= sure || lo == kBins);
+                const u64 who = __ballot(in);
+                const int at = n_kept + (int)__builtin_amdgcn_mbcnt_hi(
+                                            (uint32_t)(who >> 32),
+                                            __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
+                if (in) kept[wave][at] = v[e];
+                n_kept += __popcll(who);
+                if (is && !in && ((hi >= 0 && m >= listed) || (m >= k_from && m < k_to))) {
+                    // the list has no order: places by an LDS counter
+                    const int to = atomicAdd(&place, 1);
+                    if (to < kChunkList)
+                        chunk_list(a, row, c)[to] =
+                            (u64)order_key(v[e]) << 32 | (uint32_t)block_index(b, 4 * j + e);
+                }
             }
+        });
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        u64 sum = 0;
+        for (int i = lane; i < n_kept; i += 64) {
+            const double we = w(kept[wave][i]);
+            sum += we >= s.min_w ? row_units(we) : 0;
         }
-        if (hi < 0) continue;  // workgroup-uniform
-        const int have = __popc(mine);
-        const int upto = block_scan(have, ipart);
-        if (tid == kChunkThreads - 1) share = upto ? atomicAdd(row_count(a, row), upto) : 0;
-        __syncthreads();
-        int at = share + upto - have;
-        u64* list = row_list(a, row);
-#pragma unroll
-        for (int e = 0; e < 16; e++)
-            if (mine >> e & 1 && at < kList)
-                list[at++] = (u64)order_key(v[e]) << 32 | (uint32_t)block_index(b, e);
-        __syncthreads();
+        sum = wave_sum(sum);
+        const int seg = (b >> 10) + wave;
+        if (lane == 0 && seg * kSegment < a.n) segment_sums(a, row)[seg] = sum;
+        __builtin_amdgcn_wave_barrier();
     }
-    sum = wave_sum(sum);
     __syncthreads();
-    if (lane == 0) dpart[wave] = sum;
-    __syncthreads();
-    if (tid == 0) {
-        for (int i = 1; i < kChunkWaves; i++) sum += dpart[i];
-        row_stats(a, row)[c].sum = sum;
-    }
+    if (tid == 0) row_stats(a, row)[c].listed = place;
 }
 
 // ------------------------------------------------------------------ the cut
@@ -509,11 +580,7 @@ __device__ __forceinline__ void pick_digit(Select& s) {
     u64 h[4], sum = 0;
 #pragma unroll
     for (int i = 0; i < 4; i++) sum += h[i] = s.hist[255 - (4 * lane + i)];
-    u64 upto = sum;
-    for (int off = 1; off < 64; off <<= 1) {
-        const u64 o = __shfl_up(upto, off, 64);
-        if (lane >= off) upto += o;
-    }
+    const u64 upto = wave_scan(sum);
     const u64 left = s.left, over = __ballot(upto >= left);
     const int who = over ? __builtin_ctzll(over) : 63;
     if (lane == who) {
@@ -583,9 +650,9 @@ __device__ Cut select_cut(Select& s, u64 goal, Each each, Value value) {
 __global__ __launch_bounds__(kRowThreads) void tf_sample_draw_kernel(SampleArgs a) {
     extern __shared__ __align__(16) uint8_t lds[];
     u64* list = reinterpret_cast<u64*>(lds);                        // kList
-    u64* chunk_add = list + kList;                                  // kMaxChunks
-    Select& sel = *reinterpret_cast<Select*>(chunk_add + kMaxChunks);
-    __shared__ double wave_w[kRowWaves], table[32];
+    u64* seg_sum = list + kList;                                    // kMaxSegments
+    Select& sel = *reinterpret_cast<Select*>(seg_sum + kMaxSegments);
+    __shared__ double wave_w[kRowWaves], table[32], seg_before;
     __shared__ u64 total_w;
     __shared__ int answer;
     const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -593,11 +660,21 @@ __global__ __launch_bounds__(kRowThreads) void tf_sample_draw_kernel(SampleArgs 
     const int n = a.n;
     // everything that the workspace may hold of the row, at once
     const Settings s = settings(a, row);
-    ChunkStat mine_c{-INFINITY, 0, 0.0};
+    ChunkStat mine_c{-INFINITY, 0, 0, 0};
     if (lane < a.chunks) mine_c = row_stats(a, row)[lane];
     RowInfo info = *row_info(a, row);
     if (s.plain()) info.cut = 0;
-    const int count = min(*row_count(a, row), kList);
+    // the list's length and each chunk's place in it; too long for LDS, or a chunk's for
+    // its room: the row itself
+    int list_upto = 0, count = 0;
+    if (info.cut == 1) {
+        list_upto = wave_scan(mine_c.listed);
+        count = lane_value(list_upto, 63);
+        if (count > kList || __ballot(mine_c.listed > kChunkList)) info.cut = 2;
+    }
+    const int segments = (n + kSegment - 1) / kSegment;
+    u64 my_seg = 0;
+    if (tid < segments) my_seg = segment_sums(a, row)[tid];
     fill_exp2(table);
     const float l_max = tf_wave_max(mine_c.top);
     if (!(l_max > -INFINITY) || s.greedy) {  // nothing to draw, or nothing to choose
@@ -610,13 +687,17 @@ __global__ __launch_bounds__(kRowThreads) void tf_sample_draw_kernel(SampleArgs 
     auto units = [&](uint32_t key) { return row_units(w(key_logit(key))); };
     auto one = [](uint32_t) { return (u64)1; };
     if (tid == 0) answer = -1, total_w = 0;
-    if (tid < kMaxChunks) chunk_add[tid] = 0;
+    if (tid < segments) seg_sum[tid] = my_seg;
     __syncthreads();
 
     Cut cut{0u, kMaxVocab};
     if (info.cut == 1) {
-        const u64* src = row_list(a, row);
-        for (int i = tid; i < count; i += kRowThreads) list[i] = src[i];
+        for (int c = wave; c < a.chunks; c += kRowWaves) {
+            const int have = __builtin_amdgcn_readlane(mine_c.listed, c);
+            const int to = __builtin_amdgcn_readlane(list_upto, c) - have;
+            const u64* src = chunk_list(a, row, c);
+            for (int i = lane; i < have; i += 64) list[to + i] = src[i];
+        }
         __syncthreads();
         const float base = bin_of(l_max, s.per_l);
         auto each = [&](auto f) {
@@ -654,11 +735,11 @@ __global__ __launch_bounds__(kRowThreads) void tf_sample_draw_kernel(SampleArgs 
                 units);
             cut.within(k_cut);
         }
-        // what the list adds to each chunk
+        // what the list adds to each segment
         each([&](uint32_t key, int i) {
             if (!cut.keeps(key, i)) return;
             const double we = w(key_logit(key));
-            if (we >= s.min_w) atomicAdd(&chunk_add[i / a.chunk], row_units(we));
+            if (we >= s.min_w) atomicAdd(&seg_sum[i / kSegment], row_units(we));
         });
         __syncthreads();
     } else if (info.cut == 2) {
@@ -685,92 +766,75 @@ __global__ __launch_bounds__(kRowThreads) void tf_sample_draw_kernel(SampleArgs 
         }
     }
 
-    // ---- the running sum over chunks, then inside the one that passes u times the sum
-    auto weight_at = [&](int i) {
-        const float l = x[i];
-        if (!cut.keeps(order_key(l), i)) return 0.0;
+    // ---- the running sum over segments, then inside the one that passes u times the sum
+    const float cut_l = cut.key ? key_logit(cut.key) : -INFINITY;
+    auto weight_of = [&](float l, int i) {
+        if (!(l > cut_l || (l == cut_l && i <= cut.index))) return 0.0;
         const double v = w(l);
         return v >= s.min_w ? v : 0.0;
     };
-    int c0 = 0, c1 = n;  // the range to walk
-    double before = 0.0, total = 0.0;
-    double u = (double)a.u[row];
-    u = u > 0.0 ? u : 0.0;  // NaN: 0
-    const bool by_chunk = s.plain() ? !w.inf : info.cut != 2 && !w.inf;
-    if (by_chunk) {
-        // every wave scans the (at most 64) chunks for itself
-        double v = 0.0;
-        if (lane < a.chunks && mine_c.top > -INFINITY)
-            v = s.plain() ? mine_c.sum * w(mine_c.top)
-                          : mine_c.sum + (double)chunk_add[lane] * (1.0 / kRowUnit);
-        double upto = v;
-        for (int off = 1; off < 64; off <<= 1) {
-            const double o = __shfl_up(upto, off, 64);
-            if (lane >= off) upto += o;
-        }
-        total = __shfl(upto, 63, 64);
-        const u64 pass = __ballot(v > 0.0 && upto > u * total), any = __ballot(v > 0.0);
-        const int who = pass ? __builtin_ctzll(pass) : any ? 63 - __builtin_clzll(any) : 0;
-        before = __shfl(upto, who, 64) - __shfl(v, who, 64);
-        c0 = who * a.chunk;
-        c1 = min(c0 + a.chunk, n);
-    } else {
-        double sum = 0.0;
-        for (int i = tid; i < n; i += kRowThreads) sum += weight_at(i);
-        sum = wave_sum(sum);
-        if (lane == 0) wave_w[wave] = sum;
+    // inclusive running sum over the workgroup, and the sum
+    auto scan = [&](double v, double& all) {
+        const double upto = wave_scan(v);
         __syncthreads();
-        for (int i = 0; i < kRowWaves; i++) total += wave_w[i];
-        __syncthreads();
-    }
-    const double target = u * total;
-    constexpr int kEach = 8;
-    for (int b = c0; b < c1; b += kRowThreads * kEach) {  // kEach indices in a row a thread
-        double v[kEach], sum = 0.0;
-        int last = -1;
-#pragma unroll
-        for (int e = 0; e < kEach; e++) {
-            const int i = b + kEach * tid + e;
-            v[e] = i < c1 ? weight_at(i) : 0.0;
-            sum += v[e];
-            if (v[e] > 0.0) last = i;
-        }
-        double upto = sum;
-        for (int off = 1; off < 64; off <<= 1) {
-            const double o = __shfl_up(upto, off, 64);
-            if (lane >= off) upto += o;
-        }
         if (lane == 63) wave_w[wave] = upto;
         __syncthreads();
-        double all = 0.0, ahead = before;
+        double ahead = 0.0;
+        all = 0.0;
         for (int i = 0; i < kRowWaves; i++) {
             if (i < wave) ahead += wave_w[i];
             all += wave_w[i];
         }
-        double run = ahead + upto - sum;
-        int hit = -1;
-#pragma unroll
-        for (int e = 0; e < kEach; e++) {
-            run += v[e];
-            if (hit < 0 && v[e] > 0.0 && run > target) hit = b + kEach * tid + e;
-        }
-        // the first index that passes; where rounding leaves none, the last kept one
-        const u64 hits = __ballot(hit >= 0);
-        if (tid == 0) answer = -1, total_w = ~0ull;
+        return ahead + upto;
+    };
+    if (w.inf || info.cut == 2) {  // the segments' sums are not there: form them
         __syncthreads();
-        if (hits && lane == __builtin_ctzll(hits)) atomicMin(&total_w, (u64)hit);
-        if (last >= 0) atomicMax(&answer, last);
-        __syncthreads();
-        const u64 found = total_w;
-        const int kept = answer;
-        before += all;
-        if (found != ~0ull) {
-            if (tid == 0) a.out[row] = (int)found;
-            return;
+        for (int g = wave; g < segments; g += kRowWaves) {
+            double v = 0.0;
+            for (int i = g * kSegment + lane; i < min((g + 1) * kSegment, n); i += 64)
+                v += weight_of(x[i], i);
+            v = wave_sum(v);
+            if (lane == 0) seg_sum[g] = __builtin_bit_cast(u64, v);
         }
-        if (kept >= 0 && tid == 0) a.out[row] = kept;
         __syncthreads();
     }
+    double seg_w = 0.0;
+    if (tid < segments) {
+        const u64 b = seg_sum[tid];
+        if (w.inf || info.cut == 2) {
+            seg_w = __builtin_bit_cast(double, b);
+        } else if (s.plain()) {  // its chunk's largest -> the row's
+            const float top = row_stats(a, row)[tid * kSegment / a.chunk].top;
+            seg_w = __builtin_bit_cast(double, b) * w(top);
+        } else {
+            seg_w = (double)b * (1.0 / kRowUnit);
+        }
+    }
+    double total, upto = scan(seg_w, total);
+    double u = (double)a.u[row];
+    u = u > 0.0 ? u : 0.0;  // NaN: 0
+    const double target = u * total;
+    // the first that passes the target (rounding may leave none: the last with a weight)
+    auto choose = [&](bool passes, bool any, int at) {
+        __syncthreads();
+        if (tid == 0) answer = -1, total_w = ~0ull;
+        __syncthreads();
+        const u64 hits = __ballot(passes), has = __ballot(any);
+        if (hits && lane == __builtin_ctzll(hits)) atomicMin(&total_w, (u64)at);
+        if (has && lane == 63 - __builtin_clzll(has)) atomicMax(&answer, at);
+        __syncthreads();
+        return total_w != ~0ull ? (int)total_w : max(answer, 0);
+    };
+    const int seg = choose(seg_w > 0.0 && upto > target, seg_w > 0.0, tid);
+    if (seg == tid) seg_before = upto - seg_w;
+    const int i = seg * kSegment + tid;
+    const float l = i < n ? x[i] : -INFINITY;
+    __syncthreads();
+    const double before = seg_before, v = i < n ? weight_of(l, i) : 0.0;
+    double all;
+    upto = before + scan(v, all);
+    const int at = choose(v > 0.0 && upto > target, v > 0.0, i);
+    if (tid == 0) a.out[row] = at;
 }
 
 int chunk_of(int n_rows, int n_vocab) {
@@ -783,7 +847,7 @@ int chunk_of(int n_rows, int n_vocab) {
 }
 
 long long row_bytes_of(int chunks) {
-    return 128 + 8LL * kList + (long long)chunks * (sizeof(ChunkStat) + kBins * 12);
+    return 128 + sizeof(ChunkStat) * kMaxChunks + 8LL * (kMaxSegments + (long long)chunks * kChunkWords);
 }
 
 }  // namespace
@@ -816,7 +880,7 @@ extern "C" int tf_sample(const float* logits, int n_rows, int n_vocab, int row_s
     if (top_k || top_p || min_p)
         hipLaunchKernelGGL(tf_sample_gather_kernel, dim3(grid), dim3(kChunkThreads), 0,
                            tf_stream(stream), a);
-    constexpr int bytes = 8 * (kList + kMaxChunks) + (int)sizeof(Select);
+    constexpr int bytes = 8 * (kList + kMaxSegments) + (int)sizeof(Select);
     const int rc = tf_set_lds_limit((const void*)tf_sample_draw_kernel, bytes);
     if (rc) return rc;
     hipLaunchKernelGGL(tf_sample_draw_kernel, dim3(n_rows), dim3(kRowThreads), bytes,
