@@ -7,60 +7,120 @@
 // that rows of any magnitude keep their 7 bits.
 #include <math.h>
 
+#include "kv8.hpp"
 #include "lds_dma.hpp"
 #include "tf_common.hpp"
 #include "tf_host.hpp"
 
 #define TF_NEG_BIG (-1e30f)
 
-template <class T>
-__device__ __forceinline__ float tf_kv8_src(T v);
-template <>
-__device__ __forceinline__ float tf_kv8_src<float>(float v) { return v; }
-template <>
-__device__ __forceinline__ float tf_kv8_src<uint16_t>(uint16_t v) { return tf_h2f(v); }
+// Rows of n values (n % 32 == 0), blockIdx.y K or V.  What bounds both is their bytes,
+// so a lane moves 16 of the wider side at once; VEC false: a value a lane, for rows
+// that are not so aligned.
+typedef _Float16 tf_h2x __attribute__((ext_vector_type(2)));
 
-// One value a lane, a 32-lane half a group; blockIdx.y: K or V.
-template <class T>
-__global__ __launch_bounds__(256) void tf_kv8_write_kernel(const T* __restrict__ k,
-                                                           const T* __restrict__ v,
-                                                           long long src_stride,
-                                                           int8_t* __restrict__ k8,
-                                                           float* __restrict__ kd,
-                                                           int8_t* __restrict__ v8,
-                                                           float* __restrict__ vd, int n, int pos0,
-                                                           const int* __restrict__ pos0_dev,
-                                                           size_t count) {
-    const size_t e = (size_t)blockIdx.x * 256 + threadIdx.x;
-    if (e >= count) return;  // whole 32-lane halves: count % 32 == 0
-    const long long t = e / n;
-    const int i = (int)(e - t * n);
+struct TfKv8Rows {
+    const void *k, *v;
+    long long stride;
+    int8_t *k8, *v8;
+    float *kd, *vd;
+    int n, pos0;
+    const int* pos0_dev;
+    size_t count;  // values
+};
+
+template <bool F16, bool VEC>
+__global__ __launch_bounds__(256) void tf_kv8_write_kernel(TfKv8Rows a) {
+    constexpr int PER = !VEC ? 1 : F16 ? 8 : 4;  // values a lane
+    const size_t e = ((size_t)blockIdx.x * 256 + threadIdx.x) * PER;
+    if (e >= a.count) return;  // whole groups: count % 32 == 0
     const bool is_v = blockIdx.y == 1;
-    const long long pos = (long long)(pos0_dev ? pos0_dev[0] : pos0) + t;
-    const float x = tf_kv8_src<T>((is_v ? v : k)[t * src_stride + i]);
-    const float amax = tf_group32_max(fabsf(x));
-    const float d = amax * (1.0f / 127.0f);
-    const size_t at = (size_t)pos * n + i;
-    (is_v ? v8 : k8)[at] = (int8_t)tf_q8_value(x, amax, d);
-    if ((threadIdx.x & 31) == 0) (is_v ? vd : kd)[at >> 5] = d;
+    size_t t;
+    if (e >> 32 == 0) t = (uint32_t)e / (uint32_t)a.n;
+    else t = e / a.n;
+    const size_t i = e - t * a.n;
+    const size_t at = ((size_t)(a.pos0_dev ? a.pos0_dev[0] : a.pos0) + t) * a.n + i;
+    const size_t from = t * a.stride + i;
+    const void* src = is_v ? a.v : a.k;
+    int8_t* q = (is_v ? a.v8 : a.k8) + at;
+    float* ds = (is_v ? a.vd : a.kd) + (at >> 5);
+    if constexpr (!VEC) {
+        const float x = F16 ? tf_h2f(static_cast<const uint16_t*>(src)[from])
+                            : static_cast<const float*>(src)[from];
+        const float amax = tf_group32_max(fabsf(x));
+        const float d = amax * (1.0f / 127.0f);
+        *q = (int8_t)tf_q8_value(x, amax, d);
+        if ((threadIdx.x & 31) == 0) *ds = d;
+    } else if constexpr (F16) {
+        const tf_u32x4 b = tf_ld16(static_cast<const uint16_t*>(src) + from);
+        float x[8], amax = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            x[j] = tf_h2f(b[j >> 1] >> (16 * (j & 1)));
+            amax = fmaxf(amax, fabsf(x[j]));
+        }
+        amax = fmaxf(amax, tf_dpp<TF_DPP_QUAD_1032>(amax));
+        amax = fmaxf(amax, tf_dpp<TF_DPP_QUAD_2301>(amax));
+        const float d = amax * (1.0f / 127.0f), r = __builtin_amdgcn_rcpf(d);
+        tf_u32x2 o = {0, 0};
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            o[j >> 2] |= (uint32_t)(uint8_t)(int8_t)tf_q8_value_r(x[j], amax, d, r) << (8 * (j & 3));
+        *reinterpret_cast<tf_u32x2*>(q) = o;
+        if ((threadIdx.x & 3) == 0) *ds = d;
+    } else {
+        const tf_u32x4 b = tf_ld16(static_cast<const float*>(src) + from);
+        const float x[4] = {__uint_as_float(b.x), __uint_as_float(b.y), __uint_as_float(b.z),
+                            __uint_as_float(b.w)};
+        float d;
+        *reinterpret_cast<uint32_t*>(q) = tf_q8_quad(x, d);
+        if ((threadIdx.x & 7) == 0) *ds = d;
+    }
 }
 
-template <class T>
+template <bool F16, bool VEC>
 __global__ __launch_bounds__(256) void tf_kv8_read_kernel(const int8_t* __restrict__ k8,
                                                           const float* __restrict__ kd,
                                                           const int8_t* __restrict__ v8,
                                                           const float* __restrict__ vd,
-                                                          T* __restrict__ k, T* __restrict__ v,
+                                                          void* __restrict__ k, void* __restrict__ v,
                                                           size_t first, size_t count) {
-    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+    constexpr int PER = !VEC ? 1 : F16 ? 8 : 4;
+    const size_t i = ((size_t)blockIdx.x * 256 + threadIdx.x) * PER;
     if (i >= count) return;
     const bool is_v = blockIdx.y == 1;
     const size_t at = first + i;
-    float x = (float)(is_v ? v8 : k8)[at] * (is_v ? vd : kd)[at >> 5];
-    asm("" : "+v"(x));  // the f32 product is rounded: not fused with the conversion
-    T* out = is_v ? v : k;
-    if constexpr (sizeof(T) == 4) out[i] = x;
-    else out[i] = __builtin_bit_cast(uint16_t, (_Float16)x);
+    const int8_t* q = (is_v ? v8 : k8) + at;
+    const float d = (is_v ? vd : kd)[at >> 5];
+    uint32_t b[PER > 4 ? 2 : 1];
+    if constexpr (!VEC) {
+        b[0] = (uint8_t)*q;
+    } else {
+#pragma unroll
+        for (int j = 0; j < PER / 4; j++) b[j] = reinterpret_cast<const uint32_t*>(q)[j];
+    }
+    float x[PER];
+#pragma unroll
+    for (int j = 0; j < PER; j++) {
+        x[j] = (float)(int8_t)(b[j >> 2] >> (8 * (j & 3))) * d;
+        asm("" : "+v"(x[j]));  // the f32 product is rounded: not fused with the conversion
+    }
+    if constexpr (F16) {
+        uint16_t* out = static_cast<uint16_t*>(is_v ? v : k) + i;
+        if constexpr (VEC) {
+            tf_u32x4 o;
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                o[j] = __builtin_bit_cast(uint32_t, tf_h2x{(_Float16)x[2 * j], (_Float16)x[2 * j + 1]});
+            *reinterpret_cast<tf_u32x4*>(out) = o;
+        } else {
+            *out = __builtin_bit_cast(uint16_t, (_Float16)x[0]);
+        }
+    } else {
+        float* out = static_cast<float*>(is_v ? v : k) + i;
+        if constexpr (VEC) *reinterpret_cast<float4*>(out) = make_float4(x[0], x[1], x[2], x[3]);
+        else *out = x[0];
+    }
 }
 
 // ------------------------------------------- one token's attention
@@ -88,8 +148,6 @@ __global__ __launch_bounds__(256) void tf_kv8_read_kernel(const int8_t* __restri
 //          product.
 // LDS rows keep their 16-byte chunks xor-ed with the row (the copies' sources
 // are permuted), so that the 16 rows that half a wave reads lie in distinct banks.
-typedef _Float16 tf_h2x __attribute__((ext_vector_type(2)));
-
 template <int HD>
 struct TfKv8 {
     static constexpr int T = 32;                       // tokens per tile
@@ -504,17 +562,20 @@ extern "C" int tf_kv8_write(const void* k, const void* v, int src_type, int src_
     TF_CHECK_ARG((src_type == TF_KV_F32 || src_type == TF_KV_F16) && src_stride >= n);
     TF_CHECK_ARG(pos0_dev || (pos0 >= 0 && pos0 <= INT32_MAX - n_tok));
     const size_t count = (size_t)n_tok * n;
-    TF_CHECK_ARG((count + 255) / 256 <= UINT32_MAX / 256);
-    const dim3 grid((unsigned)((count + 255) / 256), 2);
-    if (src_type == TF_KV_F32)
-        hipLaunchKernelGGL(tf_kv8_write_kernel<float>, grid, dim3(256), 0, tf_stream(stream),
-                           (const float*)k, (const float*)v, src_stride, k8, kd, v8, vd, n, pos0,
-                           pos0_dev, count);
-    else
-        hipLaunchKernelGGL(tf_kv8_write_kernel<uint16_t>, grid, dim3(256), 0, tf_stream(stream),
-                           (const uint16_t*)k, (const uint16_t*)v, src_stride, k8, kd, v8, vd, n,
-                           pos0, pos0_dev, count);
-    return TF_LAUNCH_RESULT();
+    const bool f16 = src_type == TF_KV_F16;
+    const int el = f16 ? 2 : 4;
+    const bool vec = (((uintptr_t)k | (uintptr_t)v) & 15) == 0 && (long long)src_stride * el % 16 == 0 &&
+                     (((uintptr_t)k8 | (uintptr_t)v8) & 7) == 0;
+    const int per = 256 * (vec ? 16 / el : 1);
+    TF_CHECK_ARG((count + per - 1) / per <= UINT32_MAX / 256);
+    const dim3 grid((unsigned)((count + per - 1) / per), 2);
+    const TfKv8Rows a{k, v, src_stride, k8, v8, kd, vd, n, pos0, pos0_dev, count};
+    auto go = [&](auto kern) {
+        hipLaunchKernelGGL(kern, grid, dim3(256), 0, tf_stream(stream), a);
+        return TF_LAUNCH_RESULT();
+    };
+    if (f16) return vec ? go(tf_kv8_write_kernel<true, true>) : go(tf_kv8_write_kernel<true, false>);
+    return vec ? go(tf_kv8_write_kernel<false, true>) : go(tf_kv8_write_kernel<false, false>);
 }
 
 extern "C" int tf_kv8_read(const int8_t* k8, const float* kd, const int8_t* v8, const float* vd,
@@ -523,15 +584,19 @@ extern "C" int tf_kv8_read(const int8_t* k8, const float* kd, const int8_t* v8, 
     TF_CHECK_ARG(k && v && k8 && kd && v8 && vd && n > 0 && n % 32 == 0 && n_rows > 0 && row0 >= 0);
     TF_CHECK_ARG(dst_type == TF_KV_F32 || dst_type == TF_KV_F16);
     const size_t first = (size_t)row0 * n, count = (size_t)n_rows * n;
-    TF_CHECK_ARG((count + 255) / 256 <= UINT32_MAX / 256);
-    const dim3 grid((unsigned)((count + 255) / 256), 2);
-    if (dst_type == TF_KV_F32)
-        hipLaunchKernelGGL(tf_kv8_read_kernel<float>, grid, dim3(256), 0, tf_stream(stream), k8, kd,
-                           v8, vd, (float*)k, (float*)v, first, count);
-    else
-        hipLaunchKernelGGL(tf_kv8_read_kernel<uint16_t>, grid, dim3(256), 0, tf_stream(stream), k8,
-                           kd, v8, vd, (uint16_t*)k, (uint16_t*)v, first, count);
-    return TF_LAUNCH_RESULT();
+    const bool f16 = dst_type == TF_KV_F16;
+    const bool vec = (((uintptr_t)k | (uintptr_t)v) & 15) == 0 &&
+                     (((uintptr_t)k8 | (uintptr_t)v8) & 7) == 0;
+    const int per = 256 * (vec ? (f16 ? 8 : 4) : 1);
+    TF_CHECK_ARG((count + per - 1) / per <= UINT32_MAX / 256);
+    const dim3 grid((unsigned)((count + per - 1) / per), 2);
+    auto go = [&](auto kern) {
+        hipLaunchKernelGGL(kern, grid, dim3(256), 0, tf_stream(stream), k8, kd, v8, vd, k, v, first,
+                           count);
+        return TF_LAUNCH_RESULT();
+    };
+    if (f16) return vec ? go(tf_kv8_read_kernel<true, true>) : go(tf_kv8_read_kernel<true, false>);
+    return vec ? go(tf_kv8_read_kernel<false, true>) : go(tf_kv8_read_kernel<false, false>);
 }
 
 // One split (and one launch) where it gives each wave at most one tile: 256 tokens

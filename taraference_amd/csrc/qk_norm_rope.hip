@@ -10,6 +10,7 @@
 // angle (tf_rope_neox) is what the model files were not trained with.  Its
 // fraction of a turn is exact to 2^-32 there, and sine and cosine of that
 // fraction are f32.
+#include "kv8.hpp"
 #include "tf_common.hpp"
 #include "tf_host.hpp"
 
@@ -42,7 +43,130 @@ __device__ __forceinline__ float turns(long long pos, int i, int head_dim, doubl
     return (float)(a - rint(a));
 }
 
-// A head a wave, a workgroup a token and four heads.  y: the head in LDS.
+// head_dim 64, 128 and 256 on 16-byte aligned rows: a lane holds four values of a
+// head's first half and the four that they turn with, HD / 8 lanes a head, so every
+// access is 16 bytes a lane and the sum of squares a few DPP steps.  A workgroup takes
+// TOK tokens; their angles' sines and cosines, the same for all heads, are formed once,
+// a thread a pair, into LDS.  One token a workgroup (and 2048 / HD heads of it) where
+// there are few, four and all of their heads where the tokens alone fill the CUs.
+// Bound by its bytes: 4096 tokens of 28 + 8 heads of 128 into the 8-bit cache move 139
+// MB.
+template <int HD, Dest D, int TOK>
+__global__ __launch_bounds__(256) void tf_qk_norm_rope_vec_kernel(QkArgs a, int n_tok) {
+    constexpr int HALF = HD / 2, LPH = HD / 8, HEADS = 256 / LPH;
+    __shared__ __align__(16) float cs[2][TOK][HALF];
+    const int tid = threadIdx.x;
+    const int tok0 = blockIdx.x * TOK;
+    const int pos0 = a.pos0_dev ? a.pos0_dev[0] : a.pos0;
+    const int heads = a.n_head + (D == kRows ? 1 : 2) * a.n_kv;
+    const int item0 = TOK == 1 ? (int)blockIdx.y * HEADS : 0;
+    const int items = TOK == 1 ? min(heads, item0 + HEADS) : heads * min(TOK, n_tok - tok0);
+    const int m = tid % LPH;
+    // the lane's eight values of an item (a head of a token)
+    auto where = [&](int item, int& t, int& h, int& kind) {
+        t = TOK == 1 ? 0 : item / heads;
+        h = TOK == 1 ? item : item - t * heads;
+        kind = h < a.n_head ? 0 : h < a.n_head + a.n_kv ? 1 : 2;  // q, k, v
+        h -= kind == 0 ? 0 : kind == 1 ? a.n_head : a.n_head + a.n_kv;
+        t += tok0;
+    };
+    auto row = [&](int t, int h, int kind) {
+        const float* x = kind == 0   ? a.q + t * a.q_stride
+                         : kind == 1 ? a.k + t * a.k_stride
+                                     : a.v + t * a.v_stride;
+        return x + (size_t)h * HD + 4 * m;
+    };
+    int item = item0 + tid / LPH, t = 0, h = 0, kind = 2;
+    float4 x0 = make_float4(0.f, 0.f, 0.f, 0.f), x1 = x0;
+    if (item < items) {  // the first item's loads go out under the angles
+        where(item, t, h, kind);
+        const float* x = row(t, h, kind);
+        x0 = *reinterpret_cast<const float4*>(x);
+        x1 = *reinterpret_cast<const float4*>(x + HALF);
+    }
+    float4 wq[2], wk[2];
+    const float4 one = make_float4(1.f, 1.f, 1.f, 1.f);
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        wq[i] = a.q_norm ? *reinterpret_cast<const float4*>(a.q_norm + 4 * m + HALF * i) : one;
+        wk[i] = a.k_norm ? *reinterpret_cast<const float4*>(a.k_norm + 4 * m + HALF * i) : one;
+    }
+    for (int i = tid; i < TOK * HALF; i += 256) {
+        const int tt = i / HALF, pair = i % HALF;
+        float s, c;
+        sincospif(2.f * turns((long long)pos0 + tok0 + tt, pair, HD, a.log2_theta), &s, &c);
+        cs[0][tt][pair] = c;
+        cs[1][tt][pair] = s;
+    }
+    __syncthreads();
+    for (; item < items; item += HEADS) {
+        float v[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
+        const int t_now = t, h_now = h, kind_now = kind;
+        if (item + HEADS < items) {  // the next item's loads
+            where(item + HEADS, t, h, kind);
+            const float* x = row(t, h, kind);
+            x0 = *reinterpret_cast<const float4*>(x);
+            x1 = *reinterpret_cast<const float4*>(x + HALF);
+        }
+        if (kind_now != 2) {
+            const bool is_q = kind_now == 0;
+            if (is_q ? a.q_norm : a.k_norm) {
+                float ss = 0.f;
+#pragma unroll
+                for (int i = 0; i < 8; i++) ss = fmaf(v[i], v[i], ss);
+                if (LPH == 8) {
+                    ss += tf_dpp<TF_DPP_QUAD_1032>(ss);
+                    ss += tf_dpp<TF_DPP_QUAD_2301>(ss);
+                    ss += tf_dpp<TF_DPP_ROW_HALF_MIRROR>(ss);
+                } else {
+                    ss = tf_group_sum<LPH == 8 ? 16 : LPH>(ss);
+                }
+                const float rs = 1.0f / sqrtf(ss / (float)HD + a.eps);
+                const float4 w0 = is_q ? wq[0] : wk[0], w1 = is_q ? wq[1] : wk[1];
+                v[0] = v[0] * rs * w0.x, v[1] = v[1] * rs * w0.y;
+                v[2] = v[2] * rs * w0.z, v[3] = v[3] * rs * w0.w;
+                v[4] = v[4] * rs * w1.x, v[5] = v[5] * rs * w1.y;
+                v[6] = v[6] * rs * w1.z, v[7] = v[7] * rs * w1.w;
+            }
+            const float4 c4 = *reinterpret_cast<const float4*>(&cs[0][t_now - tok0][4 * m]);
+            const float4 s4 = *reinterpret_cast<const float4*>(&cs[1][t_now - tok0][4 * m]);
+            const float c[4] = {c4.x, c4.y, c4.z, c4.w}, s[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float y0 = v[i], y1 = v[i + 4];
+                v[i] = y0 * c[i] - y1 * s[i];
+                v[i + 4] = y0 * s[i] + y1 * c[i];
+            }
+        }
+        if (kind_now == 0 || D == kRows) {
+            float* out = kind_now == 0 ? a.q_out + ((size_t)t_now * a.n_head + h_now) * HD
+                                       : a.k_out + ((size_t)t_now * a.n_kv + h_now) * HD;
+            *reinterpret_cast<float4*>(out + 4 * m) = make_float4(v[0], v[1], v[2], v[3]);
+            *reinterpret_cast<float4*>(out + 4 * m + HALF) = make_float4(v[4], v[5], v[6], v[7]);
+            continue;
+        }
+        const size_t at = ((size_t)((long long)pos0 + t_now) * a.n_kv + h_now) * HD + 4 * m;
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const float* y = v + 4 * i;
+            const size_t o = at + HALF * i;
+            if (D == kF16) {
+                uint16_t* dst = (kind_now == 1 ? a.kc : a.vc) + o;
+                const tf_u32x2 b = {(uint32_t)tf_f2h_halfup(y[0]) | (uint32_t)tf_f2h_halfup(y[1]) << 16,
+                                    (uint32_t)tf_f2h_halfup(y[2]) | (uint32_t)tf_f2h_halfup(y[3]) << 16};
+                *reinterpret_cast<tf_u32x2*>(dst) = b;
+            } else {  // eight lanes hold a group
+                float d;
+                const uint32_t b = tf_q8_quad(y, d);
+                *reinterpret_cast<uint32_t*>((kind_now == 1 ? a.k8 : a.v8) + o) = b;
+                if ((m & 7) == 0) (kind_now == 1 ? a.kd : a.vd)[o >> 5] = d;
+            }
+        }
+    }
+}
+
+// Any other even head_dim, any alignment: a head a wave, a workgroup a token and four
+// heads.  y: the head in LDS.
 template <Dest D>
 __global__ __launch_bounds__(256) void tf_qk_norm_rope_kernel(QkArgs a) {
     __shared__ float lds[4][TF_QK_MAX_HEAD_DIM];
@@ -117,6 +241,29 @@ int launch(const QkArgs& a, int n_tok, float theta, tf_stream_t stream) {
     QkArgs b = a;
     b.log2_theta = log2((double)theta);
     const int heads = a.n_head + (D == kRows ? 1 : 2) * a.n_kv;
+    uintptr_t rows = (uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.q_norm |
+                     (uintptr_t)a.k_norm | (uintptr_t)a.q_out | (uintptr_t)a.k_out;
+    const long long strides = a.q_stride | a.k_stride | a.v_stride;
+    const uintptr_t f16 = (uintptr_t)a.kc | (uintptr_t)a.vc, i8 = (uintptr_t)a.k8 | (uintptr_t)a.v8;
+    if ((rows & 15) == 0 && strides % 4 == 0 && (f16 & 7) == 0 && (i8 & 3) == 0) {
+        auto go = [&](auto few, auto many, int hd) {
+            if (n_tok < 1024)
+                hipLaunchKernelGGL(few, dim3(n_tok, (heads * hd + 2047) / 2048), dim3(256), 0,
+                                   tf_stream(stream), b, n_tok);
+            else
+                hipLaunchKernelGGL(many, dim3((n_tok + 3) / 4), dim3(256), 0, tf_stream(stream), b,
+                                   n_tok);
+            return TF_LAUNCH_RESULT();
+        };
+        switch (a.head_dim) {
+        case 64:
+            return go(tf_qk_norm_rope_vec_kernel<64, D, 1>, tf_qk_norm_rope_vec_kernel<64, D, 4>, 64);
+        case 128:
+            return go(tf_qk_norm_rope_vec_kernel<128, D, 1>, tf_qk_norm_rope_vec_kernel<128, D, 4>, 128);
+        case 256:
+            return go(tf_qk_norm_rope_vec_kernel<256, D, 1>, tf_qk_norm_rope_vec_kernel<256, D, 4>, 256);
+        }
+    }
     hipLaunchKernelGGL(tf_qk_norm_rope_kernel<D>, dim3(n_tok, (heads + 3) / 4), dim3(256), 0,
                        tf_stream(stream), b);
     return TF_LAUNCH_RESULT();
