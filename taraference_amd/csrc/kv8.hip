@@ -35,12 +35,12 @@ __global__ __launch_bounds__(256) void tf_kv8_write_kernel(TfKv8Rows a) {
     const size_t e = ((size_t)blockIdx.x * 256 + threadIdx.x) * PER;
     if (e >= a.count) return;  // whole groups: count % 32 == 0
     const bool is_v = blockIdx.y == 1;
-    size_t t;
-    if (e >> 32 == 0) t = (uint32_t)e / (uint32_t)a.n;
-    else t = e / a.n;
-    const size_t i = e - t * a.n;
-    const size_t at = ((size_t)(a.pos0_dev ? a.pos0_dev[0] : a.pos0) + t) * a.n + i;
-    const size_t from = t * a.stride + i;
+    const size_t at = (size_t)(a.pos0_dev ? a.pos0_dev[0] : a.pos0) * a.n + e;
+    size_t from = e;  // tight rows
+    if (a.stride != a.n) {
+        const size_t t = e >> 32 == 0 ? (uint32_t)e / (uint32_t)a.n : e / a.n;
+        from += t * (a.stride - a.n);
+    }
     const void* src = is_v ? a.v : a.k;
     int8_t* q = (is_v ? a.v8 : a.k8) + at;
     float* ds = (is_v ? a.vd : a.kd) + (at >> 5);
@@ -61,12 +61,9 @@ __global__ __launch_bounds__(256) void tf_kv8_write_kernel(TfKv8Rows a) {
         }
         amax = fmaxf(amax, tf_dpp<TF_DPP_QUAD_1032>(amax));
         amax = fmaxf(amax, tf_dpp<TF_DPP_QUAD_2301>(amax));
-        const float d = amax * (1.0f / 127.0f), r = __builtin_amdgcn_rcpf(d);
-        tf_u32x2 o = {0, 0};
-#pragma unroll
-        for (int j = 0; j < 8; j++)
-            o[j >> 2] |= (uint32_t)(uint8_t)(int8_t)tf_q8_value_r(x[j], amax, d, r) << (8 * (j & 3));
-        *reinterpret_cast<tf_u32x2*>(q) = o;
+        uint32_t o[2];
+        const float d = tf_q8_words(x, amax, o);
+        *reinterpret_cast<tf_u32x2*>(q) = tf_u32x2{o[0], o[1]};
         if ((threadIdx.x & 3) == 0) *ds = d;
     } else {
         const tf_u32x4 b = tf_ld16(static_cast<const float*>(src) + from);

@@ -47,20 +47,20 @@ __device__ __forceinline__ float turns(long long pos, int i, int head_dim, doubl
 // head's first half and the four that they turn with, HD / 8 lanes a head, so every
 // access is 16 bytes a lane and the sum of squares a few DPP steps.  A workgroup takes
 // TOK tokens; their angles' sines and cosines, the same for all heads, are formed once,
-// a thread a pair, into LDS.  One token a workgroup (and 2048 / HD heads of it) where
-// there are few, four and all of their heads where the tokens alone fill the CUs.
+// a thread a pair, into LDS.  One token a workgroup (of few tokens, `share` heads of
+// one), four where they fill the CUs.
 // Bound by its bytes: 4096 tokens of 28 + 8 heads of 128 into the 8-bit cache move 139
 // MB.
 template <int HD, Dest D, int TOK>
-__global__ __launch_bounds__(256) void tf_qk_norm_rope_vec_kernel(QkArgs a, int n_tok) {
+__global__ __launch_bounds__(256) void tf_qk_norm_rope_vec_kernel(QkArgs a, int n_tok, int share) {
     constexpr int HALF = HD / 2, LPH = HD / 8, HEADS = 256 / LPH;
     __shared__ __align__(16) float cs[2][TOK][HALF];
     const int tid = threadIdx.x;
     const int tok0 = blockIdx.x * TOK;
     const int pos0 = a.pos0_dev ? a.pos0_dev[0] : a.pos0;
     const int heads = a.n_head + (D == kRows ? 1 : 2) * a.n_kv;
-    const int item0 = TOK == 1 ? (int)blockIdx.y * HEADS : 0;
-    const int items = TOK == 1 ? min(heads, item0 + HEADS) : heads * min(TOK, n_tok - tok0);
+    const int item0 = TOK == 1 ? (int)blockIdx.y * share : 0;
+    const int items = TOK == 1 ? min(heads, item0 + share) : heads * min(TOK, n_tok - tok0);
     const int m = tid % LPH;
     // the lane's eight values of an item (a head of a token)
     auto where = [&](int item, int& t, int& h, int& kind) {
@@ -148,7 +148,7 @@ __global__ __launch_bounds__(256) void tf_qk_norm_rope_vec_kernel(QkArgs a, int 
         const size_t at = ((size_t)((long long)pos0 + t_now) * a.n_kv + h_now) * HD + 4 * m;
 #pragma unroll
         for (int i = 0; i < 2; i++) {
-            const float* y = v + 4 * i;
+            const float y[4] = {v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]};
             const size_t o = at + HALF * i;
             if (D == kF16) {
                 uint16_t* dst = (kind_now == 1 ? a.kc : a.vc) + o;
@@ -247,12 +247,14 @@ int launch(const QkArgs& a, int n_tok, float theta, tf_stream_t stream) {
     const uintptr_t f16 = (uintptr_t)a.kc | (uintptr_t)a.vc, i8 = (uintptr_t)a.k8 | (uintptr_t)a.v8;
     if ((rows & 15) == 0 && strides % 4 == 0 && (f16 & 7) == 0 && (i8 & 3) == 0) {
         auto go = [&](auto few, auto many, int hd) {
+            // heads that a workgroup takes at once; all of them where the tokens are enough
+            const int share = n_tok < 128 ? 2048 / hd : heads;
             if (n_tok < 1024)
-                hipLaunchKernelGGL(few, dim3(n_tok, (heads * hd + 2047) / 2048), dim3(256), 0,
-                                   tf_stream(stream), b, n_tok);
+                hipLaunchKernelGGL(few, dim3(n_tok, (heads + share - 1) / share), dim3(256), 0,
+                                   tf_stream(stream), b, n_tok, share);
             else
                 hipLaunchKernelGGL(many, dim3((n_tok + 3) / 4), dim3(256), 0, tf_stream(stream), b,
-                                   n_tok);
+                                   n_tok, share);
             return TF_LAUNCH_RESULT();
         };
         switch (a.head_dim) {
