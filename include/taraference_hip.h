@@ -618,6 +618,36 @@ int tf_model_generate(tf_model *m, const int *forced, int n_forced, int pos0,
  * the stream. */
 int tf_model_prefill(tf_model *m, const int *tokens, int n_tok, int pos0,
                      int *next_token, tf_stream_t stream);
+/* No counterpart in the reference, whose sampler runs on the host: how a token
+ * is drawn (see tf_sample; top_k 0, top_p 1 and min_p 0 are off). */
+typedef struct tf_sampling {
+    float temperature;
+    int top_k;
+    float top_p, min_p;
+} tf_sampling;
+/* Draws *token from the logits of the last step or prefill, by u in [0, 1).
+ * n_vocab < 2^19.  Blocks on the stream. */
+int tf_model_sample(tf_model *m, const tf_sampling *how, float u, int *token,
+                    tf_stream_t stream);
+/* tf_model_generate with the continuation drawn instead of greedy: tokens[i]
+ * (i < n_gen, n_gen >= 1) comes from the logits of step n_forced - 1 + i by
+ * u[i] and is the next step's input.  The step alone is replayed from the
+ * graph. */
+int tf_model_generate_sampled(tf_model *m, const int *forced, int n_forced,
+                              int pos0, int n_gen, const tf_sampling *how,
+                              const float *u, int *tokens, int use_graph,
+                              tf_stream_t stream);
+/* No counterpart in the reference: hold the K/V cache in 8 bits (see
+ * tf_kv8_write) from here on, n_layer * max_seq * n_kv * head_dim * 2.25 bytes
+ * in place of 4.  Rows written before are lost.  Steps take path 0 with
+ * tf_qk_norm_rope_append_kv8 and tf_flash_decode_kv8 in it; prompts attend over
+ * the rows read back in f16.  head_dim 64, 128 or 256, n_head / n_kv <= 16 (else
+ * hipErrorNotSupported).  There is no way back; tf_model_set_path(1 .. 4) then
+ * returns hipErrorNotSupported and tf_model_k_cache / v_cache NULL. */
+int tf_model_use_kv8(tf_model *m);
+/* The 8-bit cache of layer li: part 0 = int8 k, 1 = f32 k scales, 2 = int8 v, 3 =
+ * f32 v scales; NULL without one. */
+const void *tf_model_kv8_cache(const tf_model *m, int li, int part);
 /* Select the kernel sequence of a step (all compute the same step):
  *   0  the reference's sequence through the operator API (cuda/layer.rs
  *      order, one launch per reference kernel);

@@ -79,6 +79,15 @@ __global__ void tf_decode_advance_kernel(int* pos, int* step, int* token, const 
     *step = s + 1;
 }
 
+// After a step's advance: the drawn token in place of the argmax, in the log and, past
+// the forced tokens, as the next input.
+__global__ void tf_decode_take_kernel(const int* drawn, const int* step, const int* n_forced,
+                                      int* token, int* log) {
+    const int s = *step;
+    log[s - 1] = *drawn;
+    if (s >= *n_forced) *token = *drawn;
+}
+
 template <class T>
 T* dev_alloc(size_t n) {
     void* p = nullptr;
@@ -104,6 +113,21 @@ struct tf_model {
     float* q8_d = nullptr;
     size_t partial_stride = 0;
     std::vector<uint16_t*> kc, vc;
+    // the 8-bit cache (tf_model_use_kv8): then kc and vc are empty, and k16 / v16 hold one
+    // layer's rows in f16 while a prompt attends over them (the earlier ones read back,
+    // its own as they are)
+    struct Kv8 {
+        int8_t *k8, *v8;
+        float *kd, *vd;
+    };
+    std::vector<Kv8> kv8;
+    uint16_t *k16 = nullptr, *v16 = nullptr;
+    int kv8_split = 0;
+    // sampling (tf_model_sample), allocated on first use: the settings and the numbers
+    // of a run, the drawn token, tf_sample's workspace
+    float *d_temp = nullptr, *d_topp = nullptr, *d_minp = nullptr, *d_u = nullptr;
+    int *d_topk = nullptr, *d_drawn = nullptr;
+    void* smp_ws = nullptr;
     // device decode state
     int *d_pos = nullptr, *d_step = nullptr, *d_token = nullptr, *d_argmax = nullptr;
     unsigned long long* d_amax_key = nullptr;
@@ -158,6 +182,11 @@ struct tf_model {
         T* p = dev_alloc<T>(n);
         allocs.push_back(p);
         return p;
+    }
+
+    void release(void* p) {
+        allocs.erase(std::find(allocs.begin(), allocs.end(), p));
+        (void)hipFree(p);
     }
 
     ~tf_model() {
@@ -222,10 +251,18 @@ struct tf_model {
                     tf::gemv(s, L.wv, xb, v, L.bv, GemvResidual::none(), gemv_partial, partial_stride);
                 }
             }
-            tf::check(tf_rope_append(q, k, v, kc[li], vc[li], c.n_head, c.n_kv, c.head_dim, pos,
-                                     pos_dev, c.rope_theta, s),
-                      "rope + append");
-            if (b32_wo_ok(L)) {  // wo merges the attention's partials itself
+            if (!kv8.empty())
+                tf::check(tf_qk_norm_rope_append_kv8(
+                              q, c.n_head * c.head_dim, k, c.n_kv * c.head_dim, v,
+                              c.n_kv * c.head_dim, nullptr, nullptr, 0.f, q, kv8[li].k8, kv8[li].kd,
+                              kv8[li].v8, kv8[li].vd, c.n_head, c.n_kv, c.head_dim, 1, pos, pos_dev,
+                              c.rope_theta, s),
+                          "rope + append kv8");
+            else
+                tf::check(tf_rope_append(q, k, v, kc[li], vc[li], c.n_head, c.n_kv, c.head_dim, pos,
+                                         pos_dev, c.rope_theta, s),
+                          "rope + append");
+            if (kv8.empty() && b32_wo_ok(L)) {  // wo merges the attention's partials itself
                 tf::check(pos_dev ? tf_flash_decode_partial_d(q, kc[li], vc[li], flash_partial,
                                                               fd.n_head, fd.n_kv, fd.head_dim,
                                                               pos_dev, 1, fd.n_split, fd.scale, s)
@@ -237,7 +274,14 @@ struct tf_model {
                                            fd.n_split, x, (int)L.wo.n_cols, (int)L.wo.col_bytes, s),
                           "merge+wo");
             } else {
-                tf::launch_attn_flash(s, fd, q, kc[li], vc[li], flash_partial, xb, pos, pos_dev);
+                if (!kv8.empty())
+                    tf::check(tf_flash_decode_kv8(q, kv8[li].k8, kv8[li].kd, kv8[li].v8, kv8[li].vd,
+                                                  flash_partial, xb, nullptr, nullptr, fd.n_head,
+                                                  fd.n_kv, fd.head_dim, pos, pos_dev, kv8_split,
+                                                  fd.scale, s),
+                              "flash kv8");
+                else
+                    tf::launch_attn_flash(s, fd, q, kc[li], vc[li], flash_partial, xb, pos, pos_dev);
                 if (!tf::try_gemv_global_q8(s, L.wo, xb, x, nullptr, GemvResidual::in_place(), q8_x,
                                             q8_d, gemv_partial, partial_stride))
                     tf::gemv(s, L.wo, xb, x, nullptr, GemvResidual::in_place(), gemv_partial,
@@ -673,13 +717,51 @@ struct tf_model {
 
     void capture() { capture_steps(1, graph, graph_exec); }
 
+    void ensure_sampling() {
+        if (smp_ws) return;
+        const long long bytes = tf_sample_ws_bytes(1, cfg.n_vocab);
+        if (bytes < 0) throw tf::HipError((int)hipErrorNotSupported, "vocabulary too large to sample");
+        d_temp = alloc<float>(1);
+        d_topp = alloc<float>(1);
+        d_minp = alloc<float>(1);
+        d_topk = alloc<int>(1);
+        d_drawn = alloc<int>(1);
+        d_u = alloc<float>(cfg.max_seq);
+        smp_ws = alloc<uint8_t>((size_t)bytes);
+    }
+    // The settings of the draws to come, and the numbers they take.  Synchronous: the
+    // host's copies may go.
+    void set_sampling(hipStream_t s, const tf_sampling& how, const float* u, int n) {
+        ensure_sampling();
+        tf::check((int)hipMemcpyAsync(d_temp, &how.temperature, sizeof(float),
+                                      hipMemcpyHostToDevice, s), "copy");
+        tf::check((int)hipMemcpyAsync(d_topk, &how.top_k, sizeof(int), hipMemcpyHostToDevice, s),
+                  "copy");
+        tf::check((int)hipMemcpyAsync(d_topp, &how.top_p, sizeof(float), hipMemcpyHostToDevice, s),
+                  "copy");
+        tf::check((int)hipMemcpyAsync(d_minp, &how.min_p, sizeof(float), hipMemcpyHostToDevice, s),
+                  "copy");
+        tf::check((int)hipMemcpyAsync(d_u, u, sizeof(float) * n, hipMemcpyHostToDevice, s), "copy");
+        tf::check((int)hipStreamSynchronize(s), "sync");
+    }
+    // *d_drawn from the current logits by number i; filters that are off cost no launch.
+    void draw(hipStream_t s, const tf_sampling& how, int i) {
+        tf::check(tf_sample(logits, 1, cfg.n_vocab, cfg.n_vocab, d_temp,
+                            how.top_k > 0 && how.top_k < cfg.n_vocab ? d_topk : nullptr,
+                            how.top_p < 1.f ? d_topp : nullptr, how.min_p > 0.f ? d_minp : nullptr,
+                            d_u + i, d_drawn, smp_ws, tf_sample_ws_bytes(1, cfg.n_vocab), s),
+                  "sample");
+    }
+
     // Runs n_forced + max(n_gen, 1) - 1 steps from position pos0 with
-    // device-resident state; tokens[i] = argmax of step n_forced - 1 + i.
+    // device-resident state; tokens[i] = argmax of step n_forced - 1 + i, or with `how`
+    // the token drawn from its logits by u[i].
     void run(hipStream_t s, const int* forced, int n_forced, int pos0, int n_gen, int* tokens,
-             bool use_graph) {
+             bool use_graph, const tf_sampling* how = nullptr, const float* u = nullptr) {
         const int total = n_forced + (n_gen > 0 ? n_gen : 1) - 1;
         if (n_forced < 1 || pos0 < 0 || pos0 + total > cfg.max_seq)
             throw tf::HipError(1, "decode range outside the KV cache");
+        if (how) set_sampling(s, *how, u, n_gen);
         std::vector<int> h(4);
         h[0] = pos0;
         h[1] = 0;
@@ -700,12 +782,22 @@ struct tf_model {
                 drop_graph();
             }
         }
+        // a step whose token is drawn ends a graph: all from the last forced one on
+        const int greedy = how ? n_forced - 1 : total;
         if (use_graph) {
             capture();
-            if (total >= kGraphSteps) capture_steps(kGraphSteps, graph_n, graph_exec_n);
+            if (greedy >= kGraphSteps) capture_steps(kGraphSteps, graph_n, graph_exec_n);
         }
         for (int i = 0; i < total;) {
-            if (use_graph && total - i >= kGraphSteps) {
+            if (i >= greedy) {
+                if (use_graph) tf::check((int)hipGraphLaunch(graph_exec, s), "graph launch");
+                else run_step(s, 0, 0, true);
+                draw(s, *how, i - greedy);
+                hipLaunchKernelGGL(tf_decode_take_kernel, dim3(1), dim3(1), 0, s, d_drawn, d_step,
+                                   d_nforced, d_token, d_log);
+                tf::check((int)hipGetLastError(), "take");
+                i++;
+            } else if (use_graph && greedy - i >= kGraphSteps) {
                 tf::check((int)hipGraphLaunch(graph_exec_n, s), "graph launch");
                 i += kGraphSteps;
             } else {
@@ -787,10 +879,22 @@ struct tf_model {
                 const int cb[3] = {(int)L.wq.col_bytes, (int)L.wk.col_bytes, (int)L.wv.col_bytes};
                 tf::check(tf_pg_qkv(w, bb, nc, cb, pf_img, E, nt, pf_ws, pf_ws_floats, &part, ts),
                           "qkv");
-                tf::check(tf_pg_qkv_post(part, L.bq, L.bk, L.bv, pf_q, kc[li], vc[li], c.n_head,
+                uint16_t *lk = k16, *lv = v16;
+                if (kv8.empty()) {
+                    lk = kc[li];
+                    lv = vc[li];
+                } else if (p0 > 0) {  // the earlier rows, as f16
+                    tf::check(tf_kv8_read(kv8[li].k8, kv8[li].kd, kv8[li].v8, kv8[li].vd, lk, lv,
+                                          TF_KV_F16, kvd, 0, p0, ts), "kv8 read");
+                }
+                tf::check(tf_pg_qkv_post(part, L.bq, L.bk, L.bv, pf_q, lk, lv, c.n_head,
                                          c.n_kv, c.head_dim, p0, nt, c.rope_theta, ts),
                           "qkv post");
-                tf::check(tf_attn_prefill_any(pf_q, kc[li], vc[li], pf_att, c.n_head, c.n_kv,
+                if (!kv8.empty())
+                    tf::check(tf_kv8_write(lk + (size_t)p0 * kvd, lv + (size_t)p0 * kvd, TF_KV_F16,
+                                           kvd, kv8[li].k8, kv8[li].kd, kv8[li].v8, kv8[li].vd, kvd,
+                                           p0, nullptr, nt, ts), "kv8 write");
+                tf::check(tf_attn_prefill_any(pf_q, lk, lv, pf_att, c.n_head, c.n_kv,
                                               c.head_dim, p0, nullptr, nt, fd.scale, ts),
                           "prefill attention");
                 tf::check(tf_pg_image(pf_att, pf_img, E, nt, ts), "image");
@@ -981,12 +1085,102 @@ extern "C" int tf_model_prefill(tf_model* m, const int* tokens, int n_tok, int p
     }
 }
 
+extern "C" int tf_model_sample(tf_model* m, const tf_sampling* how, float u, int* token,
+                               tf_stream_t stream) {
+    if (!m || !how || !token) return (int)hipErrorInvalidValue;
+    try {
+        hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+        m->set_sampling(s, *how, &u, 1);
+        m->draw(s, *how, 0);
+        tf::check((int)hipMemcpyAsync(token, m->d_drawn, sizeof(int), hipMemcpyDeviceToHost, s),
+                  "copy");
+        tf::check((int)hipStreamSynchronize(s), "sync");
+        return 0;
+    } catch (const tf::HipError& e) {
+        return e.code;
+    } catch (const std::bad_alloc&) {
+        return (int)hipErrorOutOfMemory;
+    }
+}
+
+extern "C" int tf_model_generate_sampled(tf_model* m, const int* forced, int n_forced, int pos0,
+                                         int n_gen, const tf_sampling* how, const float* u,
+                                         int* tokens, int use_graph, tf_stream_t stream) {
+    if (!m || !forced || !how || !u || !tokens || n_forced < 1 || n_gen < 1)
+        return (int)hipErrorInvalidValue;
+    for (int i = 0; i < n_forced; i++)
+        if (forced[i] < 0 || forced[i] >= m->cfg.n_vocab) return (int)hipErrorInvalidValue;
+    try {
+        m->run(reinterpret_cast<hipStream_t>(stream), forced, n_forced, pos0, n_gen, tokens,
+               use_graph != 0, how, u);
+        return 0;
+    } catch (const tf::HipError& e) {
+        return e.code;
+    } catch (const std::bad_alloc&) {
+        return (int)hipErrorOutOfMemory;
+    }
+}
+
+extern "C" int tf_model_use_kv8(tf_model* m) {
+    if (!m) return (int)hipErrorInvalidValue;
+    if (!m->kv8.empty()) return 0;
+    const tf_model_config& c = m->cfg;
+    const int hd = c.head_dim;
+    if ((hd != 64 && hd != 128 && hd != 256) || c.n_head / c.n_kv > 16)
+        return (int)hipErrorNotSupported;
+    try {
+        // everything that may fail comes before the f16 caches go
+        const size_t n = (size_t)c.max_seq * c.n_kv * hd;
+        std::vector<tf_model::Kv8> made(c.n_layer);
+        for (auto& l : made) {
+            l.k8 = m->alloc<int8_t>(n);
+            l.v8 = m->alloc<int8_t>(n);
+            l.kd = m->alloc<float>(n / 32);
+            l.vd = m->alloc<float>(n / 32);
+        }
+        const int split = tf_flash_decode_kv8_n_split(c.n_kv, hd, c.max_seq);
+        float* partial = m->alloc<float>((size_t)c.n_head * split * (2 + hd));
+        tf::check((int)hipDeviceSynchronize(), "sync");
+        m->kv8_split = split;
+        m->flash_partial = partial;
+        // one layer's f16 rows stay as the prompts' scratch
+        m->k16 = m->kc[0];
+        m->v16 = m->vc[0];
+        for (size_t i = 1; i < m->kc.size(); i++) {
+            m->release(m->kc[i]);
+            m->release(m->vc[i]);
+        }
+        m->kc.clear();
+        m->vc.clear();
+        m->path = 0;
+        m->drop_graph();
+        m->kv8 = std::move(made);
+        return 0;
+    } catch (const tf::HipError& e) {
+        return e.code;
+    } catch (const std::bad_alloc&) {
+        return (int)hipErrorOutOfMemory;
+    }
+}
+
+extern "C" const void* tf_model_kv8_cache(const tf_model* m, int li, int part) {
+    if (!m || li < 0 || li >= (int)m->kv8.size()) return nullptr;
+    const tf_model::Kv8& l = m->kv8[li];
+    switch (part) {
+    case 0: return l.k8;
+    case 1: return l.kd;
+    case 2: return l.v8;
+    case 3: return l.vd;
+    default: return nullptr;
+    }
+}
+
 extern "C" int tf_model_get_path(const tf_model* m) { return m ? m->path : -1; }
 
 extern "C" int tf_model_set_path(tf_model* m, int path) {
     if (!m || path < 0 || path > 4) return (int)hipErrorInvalidValue;
     if (path == 4 && !m->persistent_ok()) return (int)hipErrorNotSupported;
-    if (path >= 1 && !m->kquant_ok()) return (int)hipErrorNotSupported;
+    if (path >= 1 && (!m->kquant_ok() || !m->kv8.empty())) return (int)hipErrorNotSupported;
     if (m->path != path) {
         m->path = path;
         m->drop_graph();

@@ -38,6 +38,11 @@ class TfModelConfig(C.Structure):
                 ("rms_eps", C.c_float)]
 
 
+class TfSampling(C.Structure):
+    _fields_ = [("temperature", C.c_float), ("top_k", C.c_int), ("top_p", C.c_float),
+                ("min_p", C.c_float)]
+
+
 def _bind(lib):
     lib.tf_model_create.argtypes = [C.POINTER(TfModelConfig), C.POINTER(TfLayer),
                                     C.POINTER(TfMat), C.POINTER(TfMat), C.c_void_p,
@@ -64,6 +69,17 @@ def _bind(lib):
     lib.tf_model_stage_vector.restype = C.c_void_p
     lib.tf_model_q8_record.argtypes = [C.c_void_p, C.c_int, C.c_int, C.c_int]
     lib.tf_model_q8_record.restype = C.c_void_p
+    lib.tf_model_sample.argtypes = [C.c_void_p, C.POINTER(TfSampling), C.c_float,
+                                    C.POINTER(C.c_int), C.c_void_p]
+    lib.tf_model_sample.restype = C.c_int
+    lib.tf_model_generate_sampled.argtypes = [
+        C.c_void_p, C.POINTER(C.c_int), C.c_int, C.c_int, C.c_int, C.POINTER(TfSampling),
+        C.POINTER(C.c_float), C.POINTER(C.c_int), C.c_int, C.c_void_p]
+    lib.tf_model_generate_sampled.restype = C.c_int
+    lib.tf_model_use_kv8.argtypes = [C.c_void_p]
+    lib.tf_model_use_kv8.restype = C.c_int
+    lib.tf_model_kv8_cache.argtypes = [C.c_void_p, C.c_int, C.c_int]
+    lib.tf_model_kv8_cache.restype = C.c_void_p
     lib.tf_model_logits.argtypes = [C.c_void_p]
     lib.tf_model_logits.restype = C.c_void_p
     for n in ("tf_model_k_cache", "tf_model_v_cache"):
@@ -193,6 +209,12 @@ class DecodeModel:
             raise capi.HipError(f"tf_model_create returned {rc}")
         self.h = h
         self._layers = carr
+        self.kv8 = False
+        # the batched prefill takes K-quant matrices of widths that are multiples of 256
+        mats = [self.embd, self.out] + [getattr(t, n) for t in carr for n in
+                                        ("wq", "wk", "wv", "wo", "gate", "up", "down")]
+        self.prefills = (c["n_embd"] % 256 == 0 and c["n_ff"] % 256 == 0 and
+                         all(m.type in (TYPE_Q4_K, TYPE_Q6_K) for m in mats))
 
     # ---------------------------------------------------------------- upload
     def _dev(self, a: np.ndarray) -> torch.Tensor:
@@ -320,6 +342,8 @@ class DecodeModel:
 
     def kv_cache(self, layer: int, seq: int):
         """(K, V) f16 bits [seq, n_kv*head_dim] of one layer, copied to the host."""
+        if self.kv8:
+            raise capi.HipError("the cache is held in 8 bits (kv8_cache)")
         n = seq * self.cfg["n_kv"] * self.cfg["head_dim"]
         k, v = np.empty(n, np.uint16), np.empty(n, np.uint16)
         torch.cuda.synchronize()
@@ -360,6 +384,76 @@ class DecodeModel:
             return np.array([first][:n_gen], np.int32)
         rest = self.generate([first], n_gen - 1, pos0=len(prompt), use_graph=use_graph)
         return np.concatenate([[first], rest]).astype(np.int32)
+
+    # -------------------------------------------------------------- sampling
+    def sample_logits(self, u: float, temperature: float = 1.0, top_k: int = 0,
+                      top_p: float = 1.0, min_p: float = 0.0) -> int:
+        """A token drawn from the logits of the last step or prefill by the
+        number u in [0, 1); the filters as tf_sample has them."""
+        how = TfSampling(temperature, top_k, top_p, min_p)
+        tok = C.c_int()
+        rc = self.lib.tf_model_sample(self.h, C.byref(how), u, C.byref(tok), self.stream)
+        if rc != 0:
+            raise capi.HipError(f"tf_model_sample returned {rc}")
+        return tok.value
+
+    def generate_sampled(self, forced, u, temperature: float = 1.0, top_k: int = 0,
+                         top_p: float = 1.0, min_p: float = 0.0, pos0: int = 0,
+                         use_graph: bool = True):
+        """generate() with the continuation drawn: token i by the number u[i],
+        len(u) of them."""
+        forced = np.ascontiguousarray(forced, np.int32)
+        u = np.ascontiguousarray(u, np.float32)
+        how = TfSampling(temperature, top_k, top_p, min_p)
+        out = (C.c_int * max(1, len(u)))()
+        rc = self.lib.tf_model_generate_sampled(
+            self.h, (C.c_int * len(forced))(*forced.tolist()), len(forced), pos0, len(u),
+            C.byref(how), u.ctypes.data_as(C.POINTER(C.c_float)), out, int(use_graph), self.stream)
+        if rc != 0:
+            raise capi.HipError(f"tf_model_generate_sampled returned {rc}")
+        return np.array(out[:len(u)], np.int32)
+
+    def sample(self, prompt, n_gen: int, temperature: float = 1.0, top_k: int = 0,
+               top_p: float = 1.0, min_p: float = 0.0, seed: int = 0, use_graph: bool = True):
+        """A drawn continuation of `prompt` (n_gen tokens, the numbers from
+        numpy's default generator at `seed`).  The prompt runs through
+        prefill() where the weights allow it, else through the decode path."""
+        u = np.random.default_rng(seed).random(n_gen, dtype=np.float32)
+        how = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+        if n_gen < 1:
+            return np.zeros(0, np.int32)
+        if not self.prefills:
+            return self.generate_sampled(prompt, u, use_graph=use_graph, **how)
+        self.prefill(prompt, 0)
+        first = self.sample_logits(float(u[0]), **how)
+        if n_gen == 1:
+            return np.array([first], np.int32)
+        rest = self.generate_sampled([first], u[1:], pos0=len(prompt), use_graph=use_graph, **how)
+        return np.concatenate([[first], rest]).astype(np.int32)
+
+    def use_kv8(self) -> None:
+        """Hold the K/V cache in 8 bits from here on (rows written before are
+        lost, steps take path 0): 0.5625 of the f16 cache's bytes."""
+        rc = self.lib.tf_model_use_kv8(self.h)
+        if rc != 0:
+            raise capi.HipError(f"tf_model_use_kv8 returned {rc}")
+        self.kv8 = True
+
+    def kv8_cache(self, layer: int, seq: int):
+        """(k int8 [seq, n], k scales f32 [seq, n/32], v, v scales) of one
+        layer's 8-bit cache, copied to the host."""
+        n = self.cfg["n_kv"] * self.cfg["head_dim"]
+        got = []
+        torch.cuda.synchronize()
+        for part in range(4):
+            p = self.lib.tf_model_kv8_cache(self.h, layer, part)
+            if not p:
+                raise capi.HipError("no 8-bit cache (use_kv8)")
+            a = np.empty((seq, n) if part % 2 == 0 else (seq, n // 32),
+                         np.int8 if part % 2 == 0 else np.float32)
+            capi.memcpy_d2h(a, p)
+            got.append(a)
+        return tuple(got)
 
     def close(self):
         if getattr(self, "h", None):

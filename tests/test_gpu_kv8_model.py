@@ -1,0 +1,170 @@
+"""The decode runtime on the 8-bit K/V cache (tf_model_use_kv8)."""
+import ctypes as C
+
+import numpy as np
+import pytest
+import torch
+
+import _op_ref as ref
+import oracle
+from _model_ref import RefModel, prefill64
+from taraference_amd import capi, synth
+from test_gpu_model import TINY
+from test_gpu_prefill_model import calm
+
+pytestmark = pytest.mark.gpu
+
+
+class Kv8Ref(RefModel):
+    """RefModel.step on rows held in 8 bits: RoPE and attention in 64 bits, over the rows
+    that the model under test wrote.  Its rows come from activations that agree to about
+    1e-6, so a few in 10^4 values fall a step apart, and one such value moves a 128-wide
+    row by 1 / 50 / sqrt(128) = 2e-3 of it, 6e-3 of the RMS in the largest of 1000
+    logits: taken over, the logits are held as closely as those of the f16 cache."""
+
+    def __init__(self, cfg, layers, emb, max_seq):
+        super().__init__(cfg, layers, emb, 8)
+        self.apart = self.values = 0
+        n = cfg["n_kv"] * cfg["head_dim"]
+        self.rows = [[np.zeros((max_seq, n)) for _ in range(2)] for _ in layers]
+
+    def step(self, token, pos):
+        c = self.c
+        e, hd, h, kv = c["n_embd"], c["head_dim"], c["n_head"], c["n_kv"]
+        x = oracle.embed_row(self.E, 210, token, e, self.ecb)
+        for li, L in enumerate(self.L):
+            xb = oracle.rms_norm(x, L["attn_norm"], c["rms_eps"])
+            q8, d8 = self._q8(xb)
+            wq, cb = L["wq"]
+            q, k = oracle.gemv_q4k_pair(wq, L["wk"][0], q8, d8, e, h * hd, kv * hd, cb, L["bq"],
+                                        L["bk"])
+            v = oracle.gemv_q6k_f32(L["wv"][0], xb, e, kv * hd, L["wv"][1], bias=L["bv"])
+            q, k = (ref.norm_rope(a.reshape(1, -1, hd), None, 0, [pos], c["rope_theta"])[0]
+                    .astype(np.float32).reshape(1, -1) for a in (q, k))
+            k8, kd, v8, vd = (a[pos:pos + 1] for a in self.model.kv8_cache(li, pos + 1))
+            for store, row, c8, cd in zip(self.rows[li], (k, v.reshape(1, -1)), (k8, v8), (kd, vd)):
+                mine, d = ref.q8_rows(row)
+                assert (np.abs(cd - d) <= 1e-4 * d).all()
+                diff = np.abs(c8.astype(int) - mine.astype(int))
+                assert diff.max() <= 1
+                self.apart += int(diff.sum())
+                self.values += diff.size
+                store[pos] = ref.q8_values(c8, cd)[0]
+            K, V = (r[:pos + 1] for r in self.rows[li])
+            att = ref.attention(q.reshape(h, hd), K, V, kv, 1 / np.sqrt(hd))[0]
+            x = self._global_q8(L["wo"], h * hd, att.reshape(-1).astype(np.float32), False, out=x)
+            xb = oracle.rms_norm(x, L["ffn_norm"], c["rms_eps"])
+            q8, d8 = self._q8(xb)
+            g, gcb = L["gate"]
+            hid = oracle.gemv_q4k_ffn(g, L["up"][0], q8, d8, e, c["n_ff"], gcb, 1)
+            x = self._global_q8(L["down"], c["n_ff"], hid, L["down_q6k"], out=x)
+        xb = oracle.rms_norm(x, np.ones(e, np.float32), c["rms_eps"])
+        return self._global_q8((self.E, self.ecb), e, xb, True)
+
+
+def build(ci, seed, max_seq):
+    from taraference_amd.model import DecodeModel
+
+    cfg = TINY[ci]
+    rng = np.random.default_rng(seed)
+    layers = calm([synth.qwen_layer(rng, cfg, li) for li in range(cfg["n_layer"])])
+    emb = synth.qwen_embedding(rng, cfg)
+    return cfg, layers, emb, lambda: DecodeModel(dict(cfg, max_seq=max_seq), layers, emb)
+
+
+@pytest.mark.parametrize("ci", [0, 1])
+def test_steps(gpu, ci):
+    """Logits to 2e-3 of their RMS, as test_gpu_model has them over f16 rows."""
+    cfg, layers, emb, make = build(ci, 40 + ci, 48)
+    gm, rm = make(), Kv8Ref(cfg, layers, emb, 48)
+    gm.use_kv8()
+    rm.model = gm
+    assert gm.path() == 0
+    rng = np.random.default_rng(ci)
+    toks = rng.integers(0, cfg["n_vocab"], 24).tolist()
+    for pos, tok in enumerate(toks):
+        gm.forward(tok, pos)
+        got, want = gm.logits().astype(np.float64), rm.step(tok, pos).astype(np.float64)
+        assert np.abs(got - want).max() <= 2e-3 * np.sqrt(np.mean(want**2)), pos
+    assert rm.apart <= 2e-3 * rm.values  # rows agree to 1e-5 RMS: one value in 10^3
+    gm.close()
+
+
+def test_graph_replays(gpu):
+    cfg, layers, emb, make = build(1, 5, 64)
+    gm = make()
+    gm.use_kv8()
+    gm.use_kv8()  # again: nothing to do
+    prompt = list(range(5, 21))
+    eager = gm.generate(prompt, 20, use_graph=False)
+    for _ in range(3):
+        assert np.array_equal(gm.generate(prompt, 20, use_graph=True), eager)
+    gm.close()
+
+
+def put_rows(f16, gm, cfg, rows):
+    """gm's 8-bit rows 0 .. rows - 1, read back as f16, into the f16 model's cache."""
+    hip = C.CDLL("libamdhip64.so.7")
+    torch.cuda.synchronize()
+    for li in range(cfg["n_layer"]):
+        k8, kd, v8, vd = gm.kv8_cache(li, rows)
+        for q, d, dst in ((k8, kd, f16.lib.tf_model_k_cache), (v8, vd, f16.lib.tf_model_v_cache)):
+            x = (q.reshape(-1, 32).astype(np.float32) * d.reshape(-1, 1)).astype(np.float16)
+            assert hip.hipMemcpy(C.c_void_p(dst(f16.h, li)), x.ctypes.data_as(C.c_void_p),
+                                 C.c_size_t(x.nbytes), 1) == 0
+
+
+@pytest.mark.parametrize("n,more", [(40, 0), (33, 21), (1024 + 37, 11)])
+def test_prompts(gpu, n, more):
+    """A chunk of a prompt attends over its own rows as they are and over earlier ones
+    as the 8-bit cache has them: bit for bit what the f16 model gives once its earlier
+    rows are those."""
+    cfg, layers, emb, make = build(0, n, n + more + 8)
+    toks = np.random.default_rng(n).integers(0, cfg["n_vocab"], n + more).tolist()
+    f16, gm = make(), make()
+    gm.use_kv8()
+    done = 0
+    for part in (n, more):
+        if not part:
+            continue
+        tok = gm.prefill(toks[done:done + part], done)
+        for at in range(done, done + part, 1024):  # the chunks of a call
+            if at:
+                put_rows(f16, gm, cfg, at)
+            want = f16.prefill(toks[at:min(at + 1024, done + part)], at)
+        done += part
+        assert tok == want and np.array_equal(f16.logits(), gm.logits())
+    # layer 0's rows: half a step from the exact ones, which f16 and the GEMM's 2e-4 of
+    # the row's RMS (and the f32 angle, 2^-22 of a turned value a position) precede
+    K, V, _ = prefill64(cfg, layers, emb, toks)
+    k8, kd, v8, vd = gm.kv8_cache(0, n + more)
+    for q, d, want, turn in ((k8, kd, K[0], 2.0**-22), (v8, vd, V[0], 0.0)):
+        step = np.repeat(d.astype(np.float64), 32, axis=1)
+        rms = np.sqrt(np.mean(want**2, axis=1, keepdims=True))
+        near = 2e-4 * rms + np.abs(want) * 2.0**-10
+        near = near + turn * np.arange(n + more)[:, None] * np.abs(want).max(1, keepdims=True)
+        # the scale itself is as near, and so is every multiple of it up to 127
+        assert (np.abs(ref.q8_values(q, d) - want) <= 0.5 * step + 2 * near + 2.0**-20 * rms).all()
+    # and on with the decode path
+    gm.generate([1], 3, pos0=n + more)
+    f16.close()
+    gm.close()
+
+
+def test_refusals(gpu):
+    _, _, _, make = build(0, 1, 16)
+    gm = make()
+    lib, h = gm.lib, gm.h
+    assert not lib.tf_model_kv8_cache(h, 0, 0)
+    assert lib.tf_model_use_kv8(None) == 1
+    gm.use_kv8()
+    for path in (1, 2, 3, 4):
+        with pytest.raises(capi.HipError):
+            gm.set_path(path)
+    gm.set_path(0)
+    assert not lib.tf_model_k_cache(h, 0) and not lib.tf_model_v_cache(h, 0)
+    assert lib.tf_model_kv8_cache(h, 1, 3) and not lib.tf_model_kv8_cache(h, 1, 4)
+    assert not lib.tf_model_kv8_cache(h, 2, 0) and not lib.tf_model_kv8_cache(h, -1, 0)
+    with pytest.raises(capi.HipError):
+        gm.kv_cache(0, 1)
+    gm.close()
