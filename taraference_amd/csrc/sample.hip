@@ -46,14 +46,14 @@ constexpr float kPerZ = 8.f;
 constexpr int kList = 8192;         // elements of a row's list, and
 constexpr int kChunkList = 2048;    // of a chunk's part of it
 constexpr int kChunkThreads = 512, kChunkWaves = kChunkThreads / 64;
-constexpr int kBlock = 16 * kChunkThreads;  // elements that a chunk's workgroup holds at once
+constexpr int kBlock = 16 * kChunkThreads;  // elements of a chunk: its workgroup's registers
 constexpr int kMaxVocab = 1 << 19;
 constexpr int kMaxChunks = kMaxVocab / kBlock;  // 64
 constexpr int kSegment = 1024;                  // elements of a wave: what the draw walks
 constexpr int kMaxSegments = kMaxVocab / kSegment;
 constexpr int kRowThreads = 1024, kRowWaves = kRowThreads / 64;
-// Integer weights: a chunk has at most 2^17 elements, a row fewer than 2^19, so that
-// their sums stay below 2^63.
+// Integer weights: a chunk has 2^13 elements, a row fewer than 2^19, so that their sums
+// stay below 2^63.
 constexpr double kChunkUnit = 0x1p46, kRowUnit = 0x1p44;
 
 // Ordered bits of a logit: NaN lowest, -0 as +0.
@@ -78,7 +78,7 @@ struct SampleArgs {
     const float* min_p;
     const float* u;
     int* out;
-    int chunk, chunks;  // elements of a chunk, chunks of a row
+    int chunks;  // of a row
     uint8_t* ws;
     long long row_bytes;  // of the workspace
 };
@@ -108,15 +108,13 @@ __device__ __forceinline__ ChunkStat* row_stats(const SampleArgs& a, int row) {
 __device__ __forceinline__ u64* segment_sums(const SampleArgs& a, int row) {
     return reinterpret_cast<u64*>(row_stats(a, row) + kMaxChunks);
 }
-constexpr int kChunkWords = kChunkList + kBins + kBins / 2;
+constexpr int kChunkWords = kChunkList + 2 * kBins;
 __device__ __forceinline__ u64* chunk_list(const SampleArgs& a, int row, int c) {
     return segment_sums(a, row) + kMaxSegments + (size_t)c * kChunkWords;
 }
-__device__ __forceinline__ u64* chunk_weights(const SampleArgs& a, int row, int c) {
-    return chunk_list(a, row, c) + kChunkList;
-}
-__device__ __forceinline__ uint32_t* chunk_counts(const SampleArgs& a, int row, int c) {
-    return reinterpret_cast<uint32_t*>(chunk_weights(a, row, c) + kBins);
+// Its histogram as totals up to each bin: counts, then weights (kChunkUnit).
+__device__ __forceinline__ double* chunk_totals(const SampleArgs& a, int row, int c) {
+    return reinterpret_cast<double*>(chunk_list(a, row, c) + kChunkList);
 }
 static_assert(sizeof(RowInfo) <= 128 && sizeof(ChunkStat) == 16, "the workspace's layout");
 
@@ -264,6 +262,15 @@ template <class T>
 __device__ __forceinline__ T wave_sum(T v) {
     return lane_value(wave_scan(v), 63);
 }
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
+    v = max(v, dpp_or_0<0x111, 0xF>(v));
+    v = max(v, dpp_or_0<0x112, 0xF>(v));
+    v = max(v, dpp_or_0<0x114, 0xF>(v));
+    v = max(v, dpp_or_0<0x118, 0xF>(v));
+    v = max(v, dpp_or_0<0x142, 0xA>(v));
+    v = max(v, dpp_or_0<0x143, 0xC>(v));
+    return lane_value(v, 63);
+}
 
 // A block's elements: a wave holds a segment, a lane index(e) = i0 + 1024 wave + 256 (e
 // / 4) + 4 lane + e % 4; past `end`: -inf.
@@ -307,13 +314,14 @@ __global__ __launch_bounds__(kChunkThreads, 6) void tf_sample_stats_kernel(Sampl
     __shared__ u64 weight[kBins][4];
     __shared__ uint32_t count[kBins][4];
     __shared__ double table[32];
+    __shared__ u64 totals[kChunkWaves];
     __shared__ float part[kChunkWaves];
     __shared__ int first;
     const int row = blockIdx.x / a.chunks, c = blockIdx.x - row * a.chunks;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const float* x = a.logits + (size_t)row * a.stride;
-    const int i0 = c * a.chunk, end = min(i0 + a.chunk, a.n);
-    const bool many = end - i0 > kBlock;  // workgroup-uniform: the values are read again
+    const int i0 = c * kBlock, end = min(i0 + kBlock, a.n);
     float v[16];
     load_block(x, i0, end, v);
     const Settings s = settings(a, row);
@@ -323,11 +331,6 @@ __global__ __launch_bounds__(kChunkThreads, 6) void tf_sample_stats_kernel(Sampl
     float top = -INFINITY;  // fmaxf passes NaN by
 #pragma unroll
     for (int e = 0; e < 16; e++) top = fmaxf(top, v[e]);
-    for (int b = i0 + kBlock; b < end; b += kBlock) {
-        load_block(x, b, end, v);
-#pragma unroll
-        for (int e = 0; e < 16; e++) top = fmaxf(top, v[e]);
-    }
     top = tf_wave_max(top);
     if (lane == 0) part[wave] = top;
     __syncthreads();
@@ -348,65 +351,60 @@ __global__ __launch_bounds__(kChunkThreads, 6) void tf_sample_stats_kernel(Sampl
     if (!s.filtered() && !s.plain()) return;
     const RowWeight w(table, s.temp, top);
     if (s.plain()) {
-        for (int b = i0; b < end; b += kBlock) {
-            if (many) load_block(x, b, end, v);
-            double sum = 0.0;
-            if (!empty)
-                each_four(v, [&](int) {
+        double sum = 0.0;
+        if (!empty)
+            each_four(v, [&](int) {
 #pragma unroll
-                    for (int e = 0; e < 4; e++) sum += w(v[e]);
-                });
-            sum = wave_sum(sum);
-            const int seg = (b >> 10) + wave;
-            if (lane == 0 && seg * kSegment < a.n)
-                segment_sums(a, row)[seg] = __builtin_bit_cast(u64, sum);
-        }
+                for (int e = 0; e < 4; e++) sum += w(v[e]);
+            });
+        sum = wave_sum(sum);
+        const int seg = (i0 >> 10) + wave;
+        if (lane == 0 && seg * kSegment < a.n)
+            segment_sums(a, row)[seg] = __builtin_bit_cast(u64, sum);
         return;
     }
     if (!empty && !s.bad) {
         const float base = bin_of(top, s.per_l);
-        for (int b = i0; b < end; b += kBlock) {
-            if (many) load_block(x, b, end, v);
-            each_four(v, [&](int) {
+        each_four(v, [&](int) {
 #pragma unroll
-                for (int e = 0; e < 4; e++) {  // -inf and NaN add nothing
-                    const int bin = bin_below(base, bin_of(v[e], s.per_l));
-                    if (s.use_k) atomicAdd(&count[bin][lane & 3], v[e] > -INFINITY ? 1u : 0u);
-                    if (s.use_p) atomicAdd(&weight[bin][lane & 3], chunk_units(w(v[e])));
-                }
-            });
-        }
+            for (int e = 0; e < 4; e++) {  // -inf and NaN add nothing
+                const int bin = bin_below(base, bin_of(v[e], s.per_l));
+                if (s.use_k) atomicAdd(&count[bin][lane & 3], v[e] > -INFINITY ? 1u : 0u);
+                if (s.use_p) atomicAdd(&weight[bin][lane & 3], chunk_units(w(v[e])));
+            }
+        });
     }
     __syncthreads();
-    u64* gw = chunk_weights(a, row, c);
-    uint32_t* gc = chunk_counts(a, row, c);
-    // the first half of the workgroup writes counts, the second weights
-    const int bin = tid % kBins;
-    if (tid < kBins) {
-        if (s.use_k) gc[bin] = count[bin][0] + count[bin][1] + count[bin][2] + count[bin][3];
-    } else if (s.use_p) {
-        gw[bin] = weight[bin][0] + weight[bin][1] + weight[bin][2] + weight[bin][3];
-    }
+    // the first half of the workgroup adds up counts, the second weights
+    const int half = wave / (kChunkWaves / 2), bin = tid % kBins;
+    u64 sum = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) sum += half ? weight[bin][i] : count[bin][i];
+    sum = wave_scan(sum);
+    if (lane == 63) totals[wave] = sum;
+    __syncthreads();
+    for (int i = half * (kChunkWaves / 2); i < wave; i++) sum += totals[i];
+    if (half ? s.use_p : s.use_k) chunk_totals(a, row, c)[tid] = (double)sum;
 }
 
 static_assert(kChunkThreads == 2 * kBins, "a half for counts, a half for weights");
 __global__ __launch_bounds__(kChunkThreads, 6) void tf_sample_gather_kernel(SampleArgs a) {
-    __shared__ u64 n_upto[kBins], w_upto[kBins], part[kChunkWaves];  // totals up to a bin
+    __shared__ u64 n_upto[kBins], w_upto[kBins];  // the row's totals up to a bin
     __shared__ double table[32], chunk_f[kMaxChunks];
     __shared__ float kept[kChunkWaves][kSegment];
     __shared__ int chunk_shift[kMaxChunks], first[3], place;
     const int row = blockIdx.x / a.chunks, c = blockIdx.x - row * a.chunks;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const float* x = a.logits + (size_t)row * a.stride;
-    const int i0 = c * a.chunk, end = min(i0 + a.chunk, a.n);
-    const bool many = end - i0 > kBlock;  // workgroup-uniform
+    const int i0 = c * kBlock, end = min(i0 + kBlock, a.n);
     float v[16];
     load_block(x, i0, end, v);
     const Settings s = settings(a, row);
     float mine_top = -INFINITY;
     if (lane < a.chunks) mine_top = row_stats(a, row)[lane].top;
     // the workgroup's first half adds up the histograms' counts, the second their weights
-    const int half = tid / kBins, bin = tid % kBins;
+    const int half = wave / (kChunkWaves / 2), bin = tid % kBins;
     fill_exp2(table);
     if (s.greedy || s.plain()) return;
     const float l_max = tf_wave_max(mine_top);
@@ -418,43 +416,40 @@ __global__ __launch_bounds__(kChunkThreads, 6) void tf_sample_gather_kernel(Samp
         return;
     }
     const float base = bin_of(l_max, s.per_l);
-    u64* upto_of = half ? w_upto : n_upto;
-    upto_of[bin] = 0;
     if (tid < 3) first[tid] = kBins - 1;
     if (tid == 0) place = 0;
     __syncthreads();  // the table
     const RowWeight w(table, s.temp, l_max);
     int lo = kBins, hi = -1, k_bin = -1;  // min-p alone: every bin is kept for sure
     if (s.filtered()) {
-        // bin b of the row: the chunks' bins, shifted by how far their largest lies below
-        // the row's, and their weights scaled alike; what falls past the last bin goes
-        // there
+        // the row's total up to a bin: each chunk's up to the bin that lies as far below its
+        // own largest, weights scaled alike; the last bin has all there is.  Sums of rising
+        // terms in one order: they rise with the bin.
         if (wave == 0) {
             const bool any = mine_top > -INFINITY;
             chunk_f[lane] = any ? w(mine_top) * (kRowUnit / kChunkUnit) : 0.0;
-            chunk_shift[lane] = any ? bin_below(base, bin_of(mine_top, s.per_l)) : 0;
+            chunk_shift[lane] = any ? bin_below(base, bin_of(mine_top, s.per_l)) : kBins;
         }
         __syncthreads();
-        if (half ? s.use_p : s.use_k)
+        double total = 0.0;
+        if (half ? s.use_p : s.use_k) {
+            const double* of = chunk_totals(a, row, 0) + kBins * half;
             for (int c0 = 0; c0 < a.chunks; c0 += 8) {
-                u64 got[8];
+                double got[8];
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const int cc = min(c0 + i, a.chunks - 1);
-                    got[i] = half ? chunk_weights(a, row, cc)[bin] : chunk_counts(a, row, cc)[bin];
+                for (int i = 0; i < 8; i++) {  // eight loads at once
+                    const int cc = min(c0 + i, a.chunks - 1), shift = chunk_shift[cc];
+                    const int from = bin == kBins - 1 ? bin : bin - shift;
+                    got[i] = of[(size_t)cc * kChunkWords + max(from, 0)];
+                    if (c0 + i >= a.chunks || from < 0 || shift == kBins) got[i] = 0.0;
                 }
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    if (c0 + i >= a.chunks || got[i] == 0) continue;
-                    if (half) got[i] = (u64)((double)got[i] * chunk_f[c0 + i] + 0.5);
-                    atomicAdd(&upto_of[min(bin + chunk_shift[c0 + i], kBins - 1)], got[i]);
-                }
+                for (int i = 0; i < 8; i++)
+                    total += got[i] * (half ? chunk_f[min(c0 + i, a.chunks - 1)] : 1.0);
             }
-        __syncthreads();
-        u64 upto = wave_scan(upto_of[bin]);
-        if (lane == 63) part[wave] = upto;
-        __syncthreads();
-        for (int i = half * (kChunkWaves / 2); i < wave; i++) upto += part[i];
+        }
+        u64* upto_of = half ? w_upto : n_upto;
+        const u64 upto = (u64)(total + 0.5);
         upto_of[bin] = upto;
         __syncthreads();
         // the bin in which a running total reaches a goal; one thread's
@@ -508,48 +503,53 @@ __global__ __launch_bounds__(kChunkThreads, 6) void tf_sample_gather_kernel(Samp
     // the chunk's weight before bin lo, and its part of the list
     // bins as bounds on the product that bin_of() rounds down: bin b holds base - b <= l
     // per_l < base - b + 1, the last one all below
-    const float sure = lo < kBins ? base - (float)(lo - 1) : -INFINITY;
+    // (lo == kBins: what min-p may keep, a bin and the rounding of the products below it)
+    const bool min_p = lo == kBins && fabsf(base) < 1e5f, all = lo == kBins && !min_p;
+    const float sure = lo < kBins ? base - (float)(lo - 1)
+                       : min_p    ? base - 2.f + __log2f((float)s.min_w) * (0.69314718f * kPerZ)
+                                  : -INFINITY;
     const float listed = hi < kBins - 1 ? base - (float)hi : -INFINITY;
     const float k_from = k_bin < 0 ? INFINITY : k_bin < kBins - 1 ? base - (float)k_bin : -INFINITY;
     const float k_to = base - (float)(k_bin - 1);
-    for (int b = i0; b < end; b += kBlock) {
-        if (many) load_block(x, b, end, v);
-        // the segment's elements that are kept for sure, side by side in LDS: few of a
-        // lane's are, and a branch for each would form weights in every wave
-        int n_kept = 0;
-        each_four(v, [&](int j) {
+    const float low = hi >= 0 ? fminf(listed, k_from) : sure;
+    // the segment's elements that are kept for sure, side by side in LDS: few of a
+    // lane's are, and a branch for each would form weights in every wave
+    int n_kept = 0;
+    each_four(v, [&](int j) {
+        // most have nothing of the kept or listed
+        const float most = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
+        if (!all && !__ballot(most * s.per_l >= low)) return;
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const float m = v[e] * s.per_l;
-                const bool is = v[e] > -INFINITY, in = is && (m >= sure || lo == kBins);
-                const u64 who = __ballot(in);
-                const int at = n_kept + (int)__builtin_amdgcn_mbcnt_hi(
-                                            (uint32_t)(who >> 32),
-                                            __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
-                if (in) kept[wave][at] = v[e];
-                n_kept += __popcll(who);
-                if (is && !in && ((hi >= 0 && m >= listed) || (m >= k_from && m < k_to))) {
-                    // the list has no order: places by an LDS counter
-                    const int to = atomicAdd(&place, 1);
-                    if (to < kChunkList)
-                        chunk_list(a, row, c)[to] =
-                            (u64)order_key(v[e]) << 32 | (uint32_t)block_index(b, 4 * j + e);
-                }
+        for (int e = 0; e < 4; e++) {
+            const float m = v[e] * s.per_l;
+            const bool is = v[e] > -INFINITY, in = is && (all || m >= sure);
+            const u64 who = __ballot(in);
+            const int at = n_kept + (int)__builtin_amdgcn_mbcnt_hi(
+                                        (uint32_t)(who >> 32),
+                                        __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
+            if (in) kept[wave][at] = v[e];
+            n_kept += __popcll(who);
+            if (is && !in && ((hi >= 0 && m >= listed) || (m >= k_from && m < k_to))) {
+                // the list has no order: places by an LDS counter
+                const int to = atomicAdd(&place, 1);
+                if (to < kChunkList)
+                    chunk_list(a, row, c)[to] =
+                        (u64)order_key(v[e]) << 32 | (uint32_t)block_index(i0, 4 * j + e);
             }
-        });
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-        u64 sum = 0;
-        for (int i = lane; i < n_kept; i += 64) {
-            const double we = w(kept[wave][i]);
-            sum += we >= s.min_w ? row_units(we) : 0;
         }
-        sum = wave_sum(sum);
-        const int seg = (b >> 10) + wave;
-        if (lane == 0 && seg * kSegment < a.n) segment_sums(a, row)[seg] = sum;
-        __builtin_amdgcn_wave_barrier();
+    });
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    u64 sum = 0;
+    for (int i = lane; i < n_kept; i += 64) {
+        const double we = w(kept[wave][i]);
+        sum += we >= s.min_w ? row_units(we) : 0;
     }
+    sum = wave_sum(sum);
+    const int seg = (i0 >> 10) + wave;
+    if (lane == 0 && seg * kSegment < a.n) segment_sums(a, row)[seg] = sum;
+    __builtin_amdgcn_wave_barrier();
     __syncthreads();
     if (tid == 0) row_stats(a, row)[c].listed = place;
 }
@@ -570,7 +570,9 @@ struct Cut {
 struct Select {
     u64 hist[256];
     u64 left;
-    int digit;
+    u64 few[64];  // elements that are ranked directly
+    int digit, count;
+    uint32_t least, most;
 };
 
 // The largest digit d such that the total of digits >= d reaches s.left, which
@@ -629,7 +631,8 @@ __device__ Cut select_cut(Select& s, u64 goal, Each each, Value value) {
     __syncthreads();
     u64 mine = 0;
     each([&](uint32_t key, int) { mine += key == prefix; });
-    if (mine) atomicAdd(&s.hist[0], mine);
+    mine = wave_sum(mine);
+    if (mine && (tid & 63) == 0) atomicAdd(&s.hist[0], mine);
     __syncthreads();
     if (need >= s.hist[0]) return {prefix, kMaxVocab};
     __syncthreads();
@@ -647,6 +650,80 @@ __device__ Cut select_cut(Select& s, u64 goal, Each each, Value value) {
     return {prefix, (int)(~at & 0xffffffu)};
 }
 
+// The same for elements in LDS, whose keys lie close (one bin's): one pass over 256 equal
+// steps from the least key to the most leaves a handful, and a wave ranks up to 64 by
+// comparing each with all.
+template <class Each, class Value>
+__device__ Cut select_near(Select& s, u64 goal, Each each, Value value) {
+    const int tid = threadIdx.x, lane = tid & 63;
+    if (goal < 1) goal = 1;
+    __syncthreads();
+    if (tid == 0) s.count = 0, s.least = ~0u, s.most = 0, s.left = goal;
+    if (tid < 256) s.hist[tid] = 0;
+    __syncthreads();
+    uint32_t least = ~0u, most = 0;
+    int mine = 0;
+    each([&](uint32_t key, int) {
+        least = min(least, key);
+        most = max(most, key);
+        mine++;
+    });
+    // one atomic a wave: a wave's lanes on one address go one after the other
+    least = ~wave_max_u32(~least);
+    most = wave_max_u32(most);
+    mine = wave_sum(mine);
+    if (mine && lane == 0) {
+        atomicMin(&s.least, least);
+        atomicMax(&s.most, most);
+        atomicAdd(&s.count, mine);
+    }
+    __syncthreads();
+    int count = s.count;
+    uint32_t from = 0, to = ~0u;  // keys that are still in question
+    if (count > 64) {
+        const uint32_t lowest = s.least;
+        const int shift = max(24 - __builtin_clz((s.most - lowest) | 1), 0);
+        each([&](uint32_t key, int) { atomicAdd(&s.hist[(key - lowest) >> shift], value(key)); });
+        __syncthreads();
+        if (tid < 64) pick_digit(s);
+        if (tid == 0) s.count = 0;
+        __syncthreads();
+        from = lowest + ((uint32_t)s.digit << shift);
+        to = from + ((1u << shift) - 1);
+        mine = 0;
+        each([&](uint32_t key, int) { mine += key >= from && key <= to; });
+        mine = wave_sum(mine);
+        if (mine && lane == 0) atomicAdd(&s.count, mine);
+        __syncthreads();
+        count = s.count;
+        if (count > 64) return select_cut(s, goal, each, value);
+    }
+    __syncthreads();
+    if (tid == 0) s.count = 0;
+    __syncthreads();
+    each([&](uint32_t key, int index) {
+        if (key >= from && key <= to)
+            s.few[atomicAdd(&s.count, 1)] = (u64)key << 32 | (uint32_t)~index;
+    });
+    __syncthreads();
+    if (tid < 64) {
+        const u64 me = lane < count ? s.few[lane] : 0;
+        const u64 part = lane < count ? value((uint32_t)(me >> 32)) : 0;
+        u64 before = 0;
+        for (int j = 0; j < count; j++) before += lane_value(me, j) > me ? lane_value(part, j) : 0;
+        const u64 left = s.left;
+        const u64 hit = __ballot(lane < count && before < left && before + part >= left);
+        // none: the goal is past them all, to which rounding may have led
+        u64 last = ~0ull;
+        if (!hit)
+            for (int j = 0; j < count; j++) last = min(last, lane_value(me, j));
+        if (lane == 0) s.few[0] = hit ? lane_value(me, __builtin_ctzll(hit)) : last;
+    }
+    __syncthreads();
+    const u64 at = s.few[0];
+    return {(uint32_t)(at >> 32), (int)~(uint32_t)at};
+}
+
 __global__ __launch_bounds__(kRowThreads) void tf_sample_draw_kernel(SampleArgs a) {
     extern __shared__ __align__(16) uint8_t lds[];
     u64* list = reinterpret_cast<u64*>(lds);                        // kList
@@ -655,7 +732,8 @@ __global__ __launch_bounds__(kRowThreads) void tf_sample_draw_kernel(SampleArgs 
     __shared__ double wave_w[kRowWaves], table[32], seg_before;
     __shared__ u64 total_w;
     __shared__ int answer;
-    const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const float* x = a.logits + (size_t)row * a.stride;
     const int n = a.n;
     // everything that the workspace may hold of the row, at once
@@ -712,11 +790,12 @@ __global__ __launch_bounds__(kRowThreads) void tf_sample_draw_kernel(SampleArgs 
                     if (bin(key) == info.k_bin) f(key, i);
                 });
             };
-            cut = select_cut(sel, (u64)(s.k - info.k_before), in_k, one);
+            cut = select_near(sel, (u64)(s.k - info.k_before), in_k, one);
             if (s.use_p) {
                 u64 add = 0;
                 in_k([&](uint32_t key, int i) { add += cut.keeps(key, i) ? units(key) : 0; });
-                if (add) atomicAdd(&total_w, add);
+                add = wave_sum(add);
+                if (add && lane == 0) atomicAdd(&total_w, add);
                 __syncthreads();
                 kept_w = info.w_before_k + total_w;
             }
@@ -724,7 +803,7 @@ __global__ __launch_bounds__(kRowThreads) void tf_sample_draw_kernel(SampleArgs 
         if (s.use_p) {
             const u64 goal = p_goal(s, kept_w);
             const Cut k_cut = cut;
-            cut = select_cut(
+            cut = select_near(
                 sel, goal > info.w_before_lo ? goal - info.w_before_lo : 1,
                 [&](auto f) {
                     each([&](uint32_t key, int i) {
@@ -759,7 +838,8 @@ __global__ __launch_bounds__(kRowThreads) void tf_sample_draw_kernel(SampleArgs 
                 });
             };
             kept([&](uint32_t key, int) { add += units(key); });
-            if (add) atomicAdd(&total_w, add);
+            add = wave_sum(add);
+            if (add && lane == 0) atomicAdd(&total_w, add);
             __syncthreads();
             cut = select_cut(sel, p_goal(s, total_w), kept, units);
             cut.within(k_cut);
@@ -804,7 +884,7 @@ __global__ __launch_bounds__(kRowThreads) void tf_sample_draw_kernel(SampleArgs 
         if (w.inf || info.cut == 2) {
             seg_w = __builtin_bit_cast(double, b);
         } else if (s.plain()) {  // its chunk's largest -> the row's
-            const float top = row_stats(a, row)[tid * kSegment / a.chunk].top;
+            const float top = row_stats(a, row)[tid * kSegment / kBlock].top;
             seg_w = __builtin_bit_cast(double, b) * w(top);
         } else {
             seg_w = (double)b * (1.0 / kRowUnit);
@@ -837,15 +917,6 @@ __global__ __launch_bounds__(kRowThreads) void tf_sample_draw_kernel(SampleArgs 
     if (tid == 0) a.out[row] = at;
 }
 
-int chunk_of(int n_rows, int n_vocab) {
-    // Chunks of 8192 elements, the workgroup's registers; longer ones where the rows
-    // alone give every CU two, as each of them adds up the histograms of all.
-    int chunk = kBlock;
-    while (chunk < 16 * kBlock && (long long)n_rows * ((n_vocab + 2 * chunk - 1) / (2 * chunk)) >= 512)
-        chunk *= 2;
-    return chunk;
-}
-
 long long row_bytes_of(int chunks) {
     return 128 + sizeof(ChunkStat) * kMaxChunks + 8LL * (kMaxSegments + (long long)chunks * kChunkWords);
 }
@@ -854,8 +925,7 @@ long long row_bytes_of(int chunks) {
 
 extern "C" long long tf_sample_ws_bytes(int n_rows, int n_vocab) {
     if (n_rows <= 0 || n_vocab <= 0 || n_vocab >= kMaxVocab) return -1;
-    const int chunk = chunk_of(n_rows, n_vocab);
-    return n_rows * row_bytes_of((n_vocab + chunk - 1) / chunk);
+    return n_rows * row_bytes_of((n_vocab + kBlock - 1) / kBlock);
 }
 
 extern "C" int tf_sample(const float* logits, int n_rows, int n_vocab, int row_stride,
@@ -869,8 +939,7 @@ extern "C" int tf_sample(const float* logits, int n_rows, int n_vocab, int row_s
     a.logits = logits, a.stride = row_stride, a.n = n_vocab;
     a.temperature = temperature, a.top_k = top_k, a.top_p = top_p, a.min_p = min_p;
     a.u = u, a.out = out_idx;
-    a.chunk = chunk_of(n_rows, n_vocab);
-    a.chunks = (n_vocab + a.chunk - 1) / a.chunk;
+    a.chunks = (n_vocab + kBlock - 1) / kBlock;
     a.ws = static_cast<uint8_t*>(ws);
     a.row_bytes = row_bytes_of(a.chunks);
     TF_CHECK_ARG((long long)n_rows * a.chunks <= (long long)(UINT32_MAX / kRowThreads));
