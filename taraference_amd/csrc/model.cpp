@@ -1128,18 +1128,24 @@ extern "C" int tf_model_use_kv8(tf_model* m) {
     const int hd = c.head_dim;
     if ((hd != 64 && hd != 128 && hd != 256) || c.n_head / c.n_kv > 16)
         return (int)hipErrorNotSupported;
+    std::vector<void*> mine;  // given back if anything fails: all that may comes first
     try {
-        // everything that may fail comes before the f16 caches go
         const size_t n = (size_t)c.max_seq * c.n_kv * hd;
         std::vector<tf_model::Kv8> made(c.n_layer);
+        mine.reserve(4 * made.size() + 1);
+        auto room = [&](auto*& p, size_t count) {
+            p = m->alloc<std::remove_reference_t<decltype(*p)>>(count);
+            mine.push_back(p);
+        };
         for (auto& l : made) {
-            l.k8 = m->alloc<int8_t>(n);
-            l.v8 = m->alloc<int8_t>(n);
-            l.kd = m->alloc<float>(n / 32);
-            l.vd = m->alloc<float>(n / 32);
+            room(l.k8, n);
+            room(l.v8, n);
+            room(l.kd, n / 32);
+            room(l.vd, n / 32);
         }
         const int split = tf_flash_decode_kv8_n_split(c.n_kv, hd, c.max_seq);
-        float* partial = m->alloc<float>((size_t)c.n_head * split * (2 + hd));
+        float* partial;
+        room(partial, (size_t)c.n_head * split * (2 + hd));
         tf::check((int)hipDeviceSynchronize(), "sync");
         m->kv8_split = split;
         m->flash_partial = partial;
@@ -1157,8 +1163,10 @@ extern "C" int tf_model_use_kv8(tf_model* m) {
         m->kv8 = std::move(made);
         return 0;
     } catch (const tf::HipError& e) {
+        for (void* p : mine) m->release(p);
         return e.code;
     } catch (const std::bad_alloc&) {
+        for (void* p : mine) m->release(p);
         return (int)hipErrorOutOfMemory;
     }
 }

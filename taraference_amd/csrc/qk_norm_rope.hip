@@ -165,6 +165,13 @@ __global__ __launch_bounds__(256) void tf_qk_norm_rope_vec_kernel(QkArgs a, int 
     }
 }
 
+// What a wave's lanes wrote to LDS is there for each other.
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // Any other even head_dim, any alignment: a head a wave, a workgroup a token and four
 // heads.  y: the head in LDS.
 template <Dest D>
@@ -192,7 +199,7 @@ __global__ __launch_bounds__(256) void tf_qk_norm_rope_kernel(QkArgs a) {
     }
     ss = tf_group_sum<64>(ss);
     const float rs = 1.0f / sqrtf(ss / (float)hd + a.eps);
-    __builtin_amdgcn_wave_barrier();
+    wave_sync();
     if (kind != 2)
         for (int i = lane; i < half; i += 64) {
             float y0 = y[i], y1 = y[i + half];
@@ -205,7 +212,7 @@ __global__ __launch_bounds__(256) void tf_qk_norm_rope_kernel(QkArgs a) {
             y[i] = y0 * c - y1 * s;
             y[i + half] = y0 * s + y1 * c;
         }
-    __builtin_amdgcn_wave_barrier();
+    wave_sync();
     if (kind == 0 || D == kRows) {
         float* out = kind == 0 ? a.q_out + ((size_t)t * a.n_head + h) * hd
                                : a.k_out + ((size_t)t * a.n_kv + h) * hd;

@@ -679,7 +679,7 @@ __device__ Cut select_near(Select& s, u64 goal, Each each, Value value) {
     }
     __syncthreads();
     int count = s.count;
-    uint32_t from = 0, to = ~0u;  // keys that are still in question
+    uint32_t from = 0, span = ~0u;  // keys still in question: from .. from + span
     if (count > 64) {
         const uint32_t lowest = s.least;
         const int shift = max(24 - __builtin_clz((s.most - lowest) | 1), 0);
@@ -689,9 +689,9 @@ __device__ Cut select_near(Select& s, u64 goal, Each each, Value value) {
         if (tid == 0) s.count = 0;
         __syncthreads();
         from = lowest + ((uint32_t)s.digit << shift);
-        to = from + ((1u << shift) - 1);
+        span = (1u << shift) - 1;  // the end may lie past 2^32
         mine = 0;
-        each([&](uint32_t key, int) { mine += key >= from && key <= to; });
+        each([&](uint32_t key, int) { mine += key - from <= span; });
         mine = wave_sum(mine);
         if (mine && lane == 0) atomicAdd(&s.count, mine);
         __syncthreads();
@@ -702,7 +702,7 @@ __device__ Cut select_near(Select& s, u64 goal, Each each, Value value) {
     if (tid == 0) s.count = 0;
     __syncthreads();
     each([&](uint32_t key, int index) {
-        if (key >= from && key <= to)
+        if (key - from <= span)
             s.few[atomicAdd(&s.count, 1)] = (u64)key << 32 | (uint32_t)~index;
     });
     __syncthreads();

@@ -193,3 +193,46 @@ def test_split_counts(gpu):
         for hd in (64, 128, 256):
             for seq in (1, 100, 5000, 131072, 10**7):
                 assert 1 <= f(kv, hd, seq) <= 256
+
+
+@pytest.mark.parametrize("ty", ["f32", "f16"])
+@pytest.mark.parametrize("off", ["rows", "cache", "read"])
+def test_rows_off_alignment(gpu, ty, off):
+    """Sources, caches and destinations at one element past an aligned address."""
+    n, t = 96, 37
+    np_t, kv_t = (np.float32, gpu.KV_F32) if ty == "f32" else (np.float16, gpu.KV_F16)
+    x = np.random.default_rng(5).standard_normal((t, n)).astype(np_t)
+    d = dev(np.concatenate([[0], x.ravel()]).astype(np_t)) if off == "rows" else dev(x)
+    src = P(d) + (d.element_size() if off == "rows" else 0)
+    at = 1 if off == "cache" else 0
+    k8, v8 = (dev(np.full(t * n + 2, 77, np.int8)) for _ in range(2))
+    kd, vd = (dev(np.zeros(t * n // 32, np.float32)) for _ in range(2))
+    call("tf_kv8_write", src, src, kv_t, n, P(k8) + at, P(kd), P(v8) + at, P(vd), n, 0, None, t, S())
+    q, s = ref.q8_rows(x.astype(np.float32))
+    f32 = (q.reshape(-1, 32).astype(np.float32) * s.reshape(-1, 1)).ravel()
+    out = [empty(t * n + 2, torch.float32 if ty == "f32" else torch.float16).fill_(5)
+           for _ in range(2)]
+    skip = 1 if off == "read" else 0
+    call("tf_kv8_read", P(k8) + at, P(kd), P(v8) + at, P(vd), *(P(o) + skip * o.element_size()
+         for o in out), kv_t, n, 0, t, S())
+    for c8, cd, o in ((k8, kd, out[0]), (v8, vd, out[1])):
+        assert np.array_equal(host(c8)[at:at + t * n], q.ravel()) and np.array_equal(host(cd), s.ravel())
+        assert (host(c8)[:at] == 77).all() and (host(c8)[at + t * n:] == 77).all()
+        assert np.array_equal(host(o)[skip:skip + t * n], f32.astype(np_t))
+        assert (host(o)[:skip] == 5).all() and (host(o)[skip + t * n:] == 5).all()
+
+
+def test_attention_of_scales_at_any_word(gpu):
+    """Head_dim 64: the scales' arrays may start at any float."""
+    h, kv, hd, seq = 14, 2, 64, 333
+    rng = np.random.default_rng(21)
+    q = rng.standard_normal((h, hd)).astype(np.float32)
+    k8, kd = cache(rng, seq, kv * hd)
+    v8, vd = cache(rng, seq, kv * hd)
+    pad = lambda a: dev(np.concatenate([[9.0], a.ravel()]).astype(np.float32))  # noqa: E731
+    dkd, dvd = pad(kd), pad(vd)
+    for n_split in (1, 8):
+        part, out = empty(h * n_split * (2 + hd)), empty(h * hd)
+        call("tf_flash_decode_kv8", P(dev(q)), P(dev(k8)), P(dkd) + 4, P(dev(v8)), P(dvd) + 4,
+             P(part), P(out), None, None, h, kv, hd, seq - 1, None, n_split, 0.125, S())
+        check(host(out).reshape(h, hd), q, ref.q8_values(k8, kd), ref.q8_values(v8, vd), kv, 0.125)

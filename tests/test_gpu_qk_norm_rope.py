@@ -139,3 +139,50 @@ def test_angle_is_exact_far_out(gpu):
     want, size = ref.norm_rope(x.reshape(1, 1, hd), None, EPS, [pos], 1e4)
     assert (np.abs(host(qo) - want.ravel()) <= tolerance(size.ravel())).all()
     assert np.array_equal(host(qo), host(ko))
+
+
+@pytest.mark.parametrize("h,kv,hd", [(14, 2, 64), (6, 1, 128), (3, 2, 256)])
+@pytest.mark.parametrize("t", [127, 128, 1023, 1025, 1026, 1027])
+def test_many_tokens_and_in_place(gpu, h, kv, hd, t):
+    """Token counts around those at which a workgroup takes all heads, or four tokens."""
+    rng = np.random.default_rng(t)
+    q, k = (rng.standard_normal((t, n * hd)).astype(np.float32) for n in (h, kv))
+    wq, wk = (rng.standard_normal(hd).astype(np.float32) for _ in range(2))
+    dq, dk = (dev(np.concatenate([a, np.full((2, a.shape[1]), 7, np.float32)])) for a in (q, k))
+    call("tf_qk_norm_rope", P(dq), h * hd, P(dk), kv * hd, P(dev(wq)), P(dev(wk)), EPS, P(dq), P(dk),
+         h, kv, hd, t, 3, None, THETA, S())
+    for got, src, n, w in ((dq, q, h, wq), (dk, k, kv, wk)):
+        want, size = ref.norm_rope(src.reshape(t, n, hd), w, EPS, 3 + np.arange(t), THETA)
+        assert (np.abs(host(got)[:t].reshape(want.shape) - want) <= tolerance(size)).all()
+        assert (host(got)[t:] == 7).all()
+
+
+@pytest.mark.parametrize("t", [3, 1030])
+def test_caches_off_alignment(gpu, t):
+    """f16 and 8-bit rows that start one element past an aligned address equal the others."""
+    h, kv, hd = 4, 2, 128
+    n = kv * hd
+    x, row, wq, wk = inputs(np.random.default_rng(t), t, h, kv, hd)
+    d, dwq, dwk, qo = dev(x), dev(wq), dev(wk), empty(t * h * hd)
+    head = (P(d), row, P(d) + 4 * h * hd, row, P(d) + 4 * (h + kv) * hd, row, P(dwq), P(dwk), EPS,
+            P(qo))
+    tail = (h, kv, hd, t, 0, None, THETA, S())
+    v = x[:, (h + kv) * hd:(h + 2 * kv) * hd]
+    q8, d8 = ref.q8_rows(v)
+    for off in (0, 1):
+        kc, vc = (dev(np.zeros(t * n + 1, np.uint16)) for _ in range(2))
+        call("tf_qk_norm_rope_append", *head, P(kc) + 2 * off, P(vc) + 2 * off, *tail)
+        k8, v8 = (dev(np.zeros(t * n + 1, np.int8)) for _ in range(2))
+        kd, vd = (dev(np.zeros(t * n // 32, np.float32)) for _ in range(2))
+        call("tf_qk_norm_rope_append_kv8", *head, P(k8) + off, P(kd), P(v8) + off, P(vd), *tail)
+        end = off + t * n
+        assert np.array_equal(host(vc)[off:end], oracle.f32_to_f16(np.ascontiguousarray(v).ravel()))
+        assert np.array_equal(host(v8)[off:end], q8.ravel()) and np.array_equal(host(vd), d8.ravel())
+        want, size = ref.norm_rope(parts(x, h, kv, hd)[1], wk, EPS, np.arange(t), THETA)
+        want, tol = want.reshape(t, n), tolerance(size).reshape(t, n)
+        got = host(kc)[off:end].view(np.float16).astype(np.float64).reshape(t, n)
+        assert (np.abs(got - want) <= tol + 2.0**-11 * (np.abs(want) + tol) + 2.0**-25).all()
+        gd = host(kd).reshape(t, -1)
+        step = np.repeat(gd.astype(np.float64), 32, axis=1)
+        val = ref.q8_values(host(k8)[off:end].reshape(t, n), gd)
+        assert (np.abs(val - want) <= step * (0.5 + 127 * 2.0**-23) + tol).all()

@@ -144,3 +144,59 @@ def test_a_distribution(gpu):
     u = ((np.arange(n) + 0.5) / n).astype(np.float32)
     got = draw(gpu, np.tile(np.log(w).astype(np.float32), (n, 1)), u)
     assert np.array_equal(np.bincount(got, minlength=5), (w * n).astype(int))
+
+
+@pytest.mark.parametrize("n", [300, 9001, 40000])
+@pytest.mark.parametrize("t", [np.inf, 1e36, 1e32, 1e-5, 1e-30, 1e-44])
+def test_extreme_temperatures_with_filters(gpu, n, t):
+    rng = np.random.default_rng(n)
+    x = logits(rng, 6, n)
+    x[1, ::3] = -np.inf
+    x[2, ::2] = np.nan
+    x[3] = rng.uniform(-3e38, 3e38, n)
+    x[4, 5] = np.inf
+    x[5] = rng.uniform(-3e38, -1e38, n)
+    for u in (0.1, 0.8):
+        us = np.full(6, u, np.float32)
+        for a in ({"k": [n // 2] * 6}, {"p": [0.7] * 6}, {"m": [0.5] * 6},
+                  {"k": [70] * 6, "p": [0.4] * 6, "m": [1e-30] * 6}):
+            a = {"t": [t] * 6, **a}
+            assert np.array_equal(draw(gpu, x, us, **a), want(x, us, **a)), (u, a)
+
+
+def test_cut_far_below_among_both_signs(gpu):
+    """The k-th element among keys that end within 2^24 of 2^32, 32 and more below the
+    largest; u past the sum takes the last kept."""
+    x = np.full((1, 400), -np.inf, np.float32)
+    x[0, 100] = 3.3e38
+    x[0, 101:201] = np.linspace(2.69e38, 2.6e38, 100)
+    x[0, 201:301] = np.linspace(-1.5e38, -1.6e38, 100)
+    for k, last in ((51, 150), (101, 200), (102, 201), (150, 249)):
+        got = draw(gpu, x, [1.0], t=[1e36], k=[k])
+        assert got[0] == last == ref.sample(x[0], np.float32(1e36), k, 1, 0, 1.0)
+
+
+def test_min_p_alone_far_down(gpu):
+    """Bounds of min-p from its least value to one, on rows of a wide and a narrow range."""
+    rng = np.random.default_rng(12)
+    x = (np.array([[40.], [0.5], [8.]]) * rng.standard_normal((3, 20000))).astype(np.float32)
+    for m in (1e-45, 1e-38, 1e-20, 1e-7, 0.02, 0.999, 1.0):
+        for u in (0.05, 0.5, 0.97):
+            a = dict(m=[m] * 3, t=[1.0, 0.7, 3.0])
+            us = np.full(3, u, np.float32)
+            assert np.array_equal(draw(gpu, x, us, **a), want(x, us, **a)), (m, u)
+
+
+def test_long_lists(gpu):
+    """Bins that hold more than a chunk's list, a row's list, or just fewer."""
+    rng = np.random.default_rng(13)
+    n = 60000
+    x = np.full((4, n), -9.0, np.float32)
+    x[0, :2000] = 1 + 0.01 * rng.random(2000)      # within a chunk's list
+    x[1, 5000:7100] = 1 + 0.01 * rng.random(2100)  # past it
+    x[2, ::8] = 1 + 0.01 * rng.random(7500)        # of every chunk, within the row's
+    x[3, ::7] = 1 + 0.01 * rng.random(8572)        # past it
+    for u in (0.2, 0.9):
+        us = np.full(4, u, np.float32)
+        for a in ({"k": [1234] * 4}, {"p": [0.61] * 4}, {"k": [1999] * 4, "p": [0.37] * 4}):
+            assert np.array_equal(draw(gpu, x, us, **a), want(x, us, **a)), (u, a)

@@ -91,6 +91,13 @@ def test_flash_kv8(lib, bad):
     assert lib.tf_flash_decode_kv8(*{**FLASH, **bad}.values(), None) == INVALID
 
 
+@pytest.mark.parametrize("bad", [{"q": A + 4}, {"k8": A + 8}, {"v8": A + 1}, {"kd": A + 4},
+                                 {"vd": A + 8}, {"kd": A + 2, "head_dim": 64},
+                                 {"v8": A + 8, "head_dim": 64}, {"pos0": 2**31 - 1024}])
+def test_flash_kv8_alignment(lib, bad):
+    assert lib.tf_flash_decode_kv8(*{**FLASH, **bad}.values(), None) == INVALID
+
+
 SAMPLE = dict(logits=A, n_rows=2, n_vocab=1000, row_stride=1000, temperature=None, top_k=None,
               top_p=None, min_p=None, u=A, out=A, ws=A, ws_bytes=1 << 30)
 
