@@ -90,6 +90,7 @@ struct RowInfo {
     u64 w_before_k, w_before_lo, w_all;  // weights in bins before k_bin, before lo, in all
     int cut;                    // 0: no cut, kept is what min-p keeps; 1: the list; 2: the row itself
     int use_k;                  // top-k cuts something
+    int wide;                   // segments' sums are of kWide, in the first one's place
 };
 struct ChunkStat {
     float top;    // the largest logit
@@ -103,16 +104,19 @@ __device__ __forceinline__ RowInfo* row_info(const SampleArgs& a, int row) {
 __device__ __forceinline__ ChunkStat* row_stats(const SampleArgs& a, int row) {
     return reinterpret_cast<ChunkStat*>(a.ws + row * a.row_bytes + 128);
 }
-// Of each segment: the sum of its weights, of its chunk's largest (no filter; f64), or
-// of the row's, of what is kept for sure (kRowUnit).
+// Of each segment (or kWide): the sum of its weights, of its chunk's largest (no filter;
+// f64), or of the row's, of what is kept for sure (kRowUnit).
 __device__ __forceinline__ u64* segment_sums(const SampleArgs& a, int row) {
     return reinterpret_cast<u64*>(row_stats(a, row) + kMaxChunks);
 }
-constexpr int kChunkWords = kChunkList + 2 * kBins;
+constexpr int kParts = 2;  // of a chunk, for its histogram
+constexpr int kWide = kBlock / kSegment / kParts;  // segments of a part
+constexpr int kChunkWords = kChunkList + (1 + kParts) * kBins;
 __device__ __forceinline__ u64* chunk_list(const SampleArgs& a, int row, int c) {
     return segment_sums(a, row) + kMaxSegments + (size_t)c * kChunkWords;
 }
-// Its histogram as totals up to each bin: counts, then weights (kChunkUnit).
+// Its histogram as totals up to each bin: counts, then the weights (kChunkUnit) of its
+// first part and of all.
 __device__ __forceinline__ double* chunk_totals(const SampleArgs& a, int row, int c) {
     return reinterpret_cast<double*>(chunk_list(a, row, c) + kChunkList);
 }
@@ -129,16 +133,21 @@ struct Settings {
     __device__ bool plain() const { return !use_k && !use_p && !(min_w > 0.0); }
 };
 __device__ __forceinline__ Settings settings(const SampleArgs& a, int row) {
-    // one value a workgroup: kept scalar, so that branches on them are
+    // one value a workgroup, read by scalar loads: they wait for no vector load, and
+    // branches on them are scalar too
+    auto at = [row](auto* p, auto off) {
+        typedef const __attribute__((address_space(4))) decltype(off) Const;
+        return p ? ((Const*)(uintptr_t)p)[row] : off;
+    };
     auto uni = [](float v) { return tf_readlane(v, 0); };
     Settings s;
-    s.temp = uni(a.temperature ? a.temperature[row] : 1.f);
+    s.temp = uni(at(a.temperature, 1.f));
     s.greedy = !(s.temp > 0.f);
-    s.k = __builtin_amdgcn_readfirstlane(a.top_k ? a.top_k[row] : 0);
+    s.k = __builtin_amdgcn_readfirstlane(at(a.top_k, 0));
     s.use_k = s.k > 0 && s.k < a.n;
-    s.p = uni(a.top_p ? a.top_p[row] : 1.f);
+    s.p = uni(at(a.top_p, 1.f));
     s.use_p = s.p < 1.f;
-    const float m = uni(a.min_p ? a.min_p[row] : 0.f);
+    const float m = uni(at(a.min_p, 0.f));
     s.min_w = m > 0.f ? fmin((double)m, 1.0) : 0.0;
     s.per_l = uni(kPerZ / s.temp);
     s.bad = !(s.temp >= 1e-6f);
@@ -310,11 +319,13 @@ __device__ __forceinline__ void each_four(float (&v)[16], F f) {
 }
 
 __global__ __launch_bounds__(kChunkThreads, 6) void tf_sample_stats_kernel(SampleArgs a) {
-    // four of each bin, by lane: half of a wave's elements may share one
-    __shared__ u64 weight[kBins][4];
-    __shared__ uint32_t count[kBins][4];
+    // several histograms, by lane (weights: and by part): half of a wave's elements may
+    // share a bin.  A wave's neighbouring bins lie in neighbouring banks, those of its other
+    // copies half of the banks further.
+    __shared__ u64 weight[2 * kParts][kBins + 16];
+    __shared__ uint32_t count[4][kBins + 16];
     __shared__ double table[32];
-    __shared__ u64 totals[kChunkWaves];
+    __shared__ u64 totals[kParts][kChunkWaves];
     __shared__ float part[kChunkWaves];
     __shared__ int first;
     const int row = blockIdx.x / a.chunks, c = blockIdx.x - row * a.chunks;
@@ -326,7 +337,8 @@ __global__ __launch_bounds__(kChunkThreads, 6) void tf_sample_stats_kernel(Sampl
     load_block(x, i0, end, v);
     const Settings s = settings(a, row);
     fill_exp2(table);
-    for (int i = tid; i < 4 * kBins; i += kChunkThreads) weight[0][i] = 0, count[0][i] = 0;
+    for (int i = tid; i < 4 * (kBins + 16); i += kChunkThreads) count[0][i] = 0;
+    for (int i = tid; i < 2 * kParts * (kBins + 16); i += kChunkThreads) weight[0][i] = 0;
     if (tid == 0) first = a.n;
     float top = -INFINITY;  // fmaxf passes NaN by
 #pragma unroll
@@ -365,34 +377,47 @@ __global__ __launch_bounds__(kChunkThreads, 6) void tf_sample_stats_kernel(Sampl
     }
     if (!empty && !s.bad) {
         const float base = bin_of(top, s.per_l);
+        const int copy = 2 * (wave / (kChunkWaves / kParts)) + (lane & 1);
         each_four(v, [&](int) {
 #pragma unroll
             for (int e = 0; e < 4; e++) {  // -inf and NaN add nothing
                 const int bin = bin_below(base, bin_of(v[e], s.per_l));
-                if (s.use_k) atomicAdd(&count[bin][lane & 3], v[e] > -INFINITY ? 1u : 0u);
-                if (s.use_p) atomicAdd(&weight[bin][lane & 3], chunk_units(w(v[e])));
+                if (s.use_k) atomicAdd(&count[lane & 3][bin], v[e] > -INFINITY ? 1u : 0u);
+                if (s.use_p) atomicAdd(&weight[copy][bin], chunk_units(w(v[e])));
             }
         });
     }
     __syncthreads();
     // the first half of the workgroup adds up counts, the second weights
     const int half = wave / (kChunkWaves / 2), bin = tid % kBins;
-    u64 sum = 0;
+    u64 sum[kParts];
 #pragma unroll
-    for (int i = 0; i < 4; i++) sum += half ? weight[bin][i] : count[bin][i];
-    sum = wave_scan(sum);
-    if (lane == 63) totals[wave] = sum;
+    for (int q = 0; q < kParts; q++) {
+        sum[q] = q ? sum[q - 1] : 0;
+        sum[q] += half ? weight[2 * q][bin] + weight[2 * q + 1][bin]
+                       : count[2 * q][bin] + count[2 * q + 1][bin];
+    }
+#pragma unroll
+    for (int q = 0; q < kParts; q++) {
+        sum[q] = wave_scan(sum[q]);
+        if (lane == 63) totals[q][wave] = sum[q];
+    }
     __syncthreads();
-    for (int i = half * (kChunkWaves / 2); i < wave; i++) sum += totals[i];
-    if (half ? s.use_p : s.use_k) chunk_totals(a, row, c)[tid] = (double)sum;
+    double* to = chunk_totals(a, row, c) + bin;
+#pragma unroll
+    for (int q = 0; q < kParts; q++) {
+        for (int i = half * (kChunkWaves / 2); i < wave; i++) sum[q] += totals[q][i];
+        if (half && s.use_p) to[(1 + q) * kBins] = (double)sum[q];
+    }
+    if (!half && s.use_k) to[0] = (double)sum[kParts - 1];
 }
 
 static_assert(kChunkThreads == 2 * kBins, "a half for counts, a half for weights");
 __global__ __launch_bounds__(kChunkThreads, 6) void tf_sample_gather_kernel(SampleArgs a) {
     __shared__ u64 n_upto[kBins], w_upto[kBins];  // the row's totals up to a bin
-    __shared__ double table[32], chunk_f[kMaxChunks];
+    __shared__ double table[32];
     __shared__ float kept[kChunkWaves][kSegment];
-    __shared__ int chunk_shift[kMaxChunks], first[3], place;
+    __shared__ int first[3], place;
     const int row = blockIdx.x / a.chunks, c = blockIdx.x - row * a.chunks;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -420,32 +445,34 @@ __global__ __launch_bounds__(kChunkThreads, 6) void tf_sample_gather_kernel(Samp
     if (tid == 0) place = 0;
     __syncthreads();  // the table
     const RowWeight w(table, s.temp, l_max);
-    int lo = kBins, hi = -1, k_bin = -1;  // min-p alone: every bin is kept for sure
+    int lo = kBins, hi = -1, k_bin = -1;  // min-p alone: no cut by bins
+    int list_from = kBins;
+    // of chunk `lane`: how far its bins lie below the row's, and its weights' scale
+    const bool any = mine_top > -INFINITY;
+    const int lane_shift = any ? bin_below(base, bin_of(mine_top, s.per_l)) : kBins;
+    const double lane_f = any ? w(mine_top) * (kRowUnit / kChunkUnit) : 0.0;
     if (s.filtered()) {
         // the row's total up to a bin: each chunk's up to the bin that lies as far below its
         // own largest, weights scaled alike; the last bin has all there is.  Sums of rising
         // terms in one order: they rise with the bin.
-        if (wave == 0) {
-            const bool any = mine_top > -INFINITY;
-            chunk_f[lane] = any ? w(mine_top) * (kRowUnit / kChunkUnit) : 0.0;
-            chunk_shift[lane] = any ? bin_below(base, bin_of(mine_top, s.per_l)) : kBins;
-        }
-        __syncthreads();
         double total = 0.0;
         if (half ? s.use_p : s.use_k) {
-            const double* of = chunk_totals(a, row, 0) + kBins * half;
-            for (int c0 = 0; c0 < a.chunks; c0 += 8) {
-                double got[8];
+            constexpr int kAtOnce = 10;
+            const double* of = chunk_totals(a, row, 0) + kParts * kBins * half;
+            for (int c0 = 0; c0 < a.chunks; c0 += kAtOnce) {
+                double got[kAtOnce];
 #pragma unroll
-                for (int i = 0; i < 8; i++) {  // eight loads at once
-                    const int cc = min(c0 + i, a.chunks - 1), shift = chunk_shift[cc];
+                for (int i = 0; i < kAtOnce; i++) {  // all loads at once
+                    const int cc = min(c0 + i, a.chunks - 1);
+                    const int shift = __builtin_amdgcn_readlane(lane_shift, cc);
                     const int from = bin == kBins - 1 ? bin : bin - shift;
-                    got[i] = of[(size_t)cc * kChunkWords + max(from, 0)];
-                    if (c0 + i >= a.chunks || from < 0 || shift == kBins) got[i] = 0.0;
+                    got[i] = (of + (size_t)cc * kChunkWords)[(uint32_t)max(from, 0)];
+                    if (from < 0) got[i] = 0.0;
                 }
 #pragma unroll
-                for (int i = 0; i < 8; i++)
-                    total += got[i] * (half ? chunk_f[min(c0 + i, a.chunks - 1)] : 1.0);
+                for (int i = 0; i < kAtOnce; i++)
+                    if (c0 + i < a.chunks)
+                        total += got[i] * (half ? lane_value(lane_f, c0 + i) : 1.0);
             }
         }
         u64* upto_of = half ? w_upto : n_upto;
@@ -484,12 +511,16 @@ __global__ __launch_bounds__(kChunkThreads, 6) void tf_sample_gather_kernel(Samp
             info.cut = 1;
             info.w_before_lo = lo ? w_upto[lo - 1] : 0;
             auto in_bins = [&](int b0, int b1) { return n_upto[b1] - (b0 ? n_upto[b0 - 1] : 0); };
+            // the bins in which min-p's bound lies: its distance below the largest, in bins, to
+            // a bin and the rounding of the products that place an element
+            const float depth = s.min_w > 0.0 ? -__log2f((float)s.min_w) * (0.69314718f * kPerZ)
+                                              : INFINITY;
+            const int first_m = (int)fminf(fmaxf(ceilf(depth - 1.7f), 0.f), (float)kBins);
+            const bool m_first = depth + 1.7f < (float)lo;
+            list_from = min(lo, first_m);
             // with top-k the list's length is known here; else the draw finds it too long
-            const u64 listed = in_bins(lo, hi) + (k_bin > hi ? in_bins(k_bin, k_bin) : 0);
-            // min-p above the first listed bin (by a bin and the rounding of the bins'
-            // products): the cuts are past it
-            if (fabsf(base) < 1e5f && lo > 2 &&
-                s.min_w > exp2_neg((2 - lo) * (1.44269504088896340736 / kPerZ), table)) {
+            const u64 listed = in_bins(list_from, hi) + (k_bin > hi ? in_bins(k_bin, k_bin) : 0);
+            if (m_first) {  // the other cuts are past it
                 info.cut = 0;
                 lo = kBins, hi = -1, k_bin = -1;
             } else if (listed > kList) {
@@ -497,21 +528,56 @@ __global__ __launch_bounds__(kChunkThreads, 6) void tf_sample_gather_kernel(Samp
             }
         }
     }
+    // the weights of bins that are kept for sure are in the histograms, if top-p took them
+    info.wide = info.cut == 1 && s.use_p;
     info.lo = lo, info.hi = hi, info.k_bin = k_bin;
     if (c == 0 && tid == 0) *row_info(a, row) = info;
     if (info.cut == 2) return;
-    // the chunk's weight before bin lo, and its part of the list
+    // the chunk's part of the list, and its weight before it
     // bins as bounds on the product that bin_of() rounds down: bin b holds base - b <= l
     // per_l < base - b + 1, the last one all below
-    // (lo == kBins: what min-p may keep, a bin and the rounding of the products below it)
+    // (min-p alone: what it may keep, a bin and the rounding of the products below it)
     const bool min_p = lo == kBins && fabsf(base) < 1e5f, all = lo == kBins && !min_p;
-    const float sure = lo < kBins ? base - (float)(lo - 1)
+    const float sure = lo < kBins ? base - (float)(list_from - 1)
                        : min_p    ? base - 2.f + __log2f((float)s.min_w) * (0.69314718f * kPerZ)
                                   : -INFINITY;
     const float listed = hi < kBins - 1 ? base - (float)hi : -INFINITY;
     const float k_from = k_bin < 0 ? INFINITY : k_bin < kBins - 1 ? base - (float)k_bin : -INFINITY;
     const float k_to = base - (float)(k_bin - 1);
     const float low = hi >= 0 ? fminf(listed, k_from) : sure;
+    auto in_list = [&](float m) {
+        return m < sure && ((hi >= 0 && m >= listed) || (m >= k_from && m < k_to));
+    };
+    auto put = [&](float l, int e) {  // the list has no order: places by an LDS counter
+        const int to = atomicAdd(&place, 1);
+        if (to < kChunkList)
+            chunk_list(a, row, c)[to] = (u64)order_key(l) << 32 | (uint32_t)block_index(i0, e);
+    };
+    if (info.wide) {
+        uint32_t which = 0;
+#pragma unroll
+        for (int e = 0; e < 16; e++)
+            which |= v[e] > -INFINITY && in_list(v[e] * s.per_l) ? 1u << e : 0;
+        for (; which; which &= which - 1) {  // few: read again
+            const int e = __builtin_ctz(which);
+            put(x[block_index(i0, e)], e);
+        }
+        if (tid < kParts) {  // a part's total is what it adds to those before it
+            const double* of = chunk_totals(a, row, c) + kBins;
+            const int from = list_from - 1 - __builtin_amdgcn_readlane(lane_shift, c);
+            double w_q = 0.0;
+            if (from >= 0)
+                w_q = (of[tid * kBins + from] - (tid ? of[(tid - 1) * kBins + from] : 0.0)) *
+                      lane_value(lane_f, c);
+            u64* to = segment_sums(a, row) + c * (kBlock / kSegment) + kWide * tid;
+            to[0] = (u64)(w_q + 0.5);
+#pragma unroll
+            for (int i = 1; i < kWide; i++) to[i] = 0;
+        }
+        __syncthreads();
+        if (tid == 0) row_stats(a, row)[c].listed = place;
+        return;
+    }
     // the segment's elements that are kept for sure, side by side in LDS: few of a
     // lane's are, and a branch for each would form weights in every wave
     int n_kept = 0;
@@ -529,13 +595,7 @@ __global__ __launch_bounds__(kChunkThreads, 6) void tf_sample_gather_kernel(Samp
                                         __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
             if (in) kept[wave][at] = v[e];
             n_kept += __popcll(who);
-            if (is && !in && ((hi >= 0 && m >= listed) || (m >= k_from && m < k_to))) {
-                // the list has no order: places by an LDS counter
-                const int to = atomicAdd(&place, 1);
-                if (to < kChunkList)
-                    chunk_list(a, row, c)[to] =
-                        (u64)order_key(v[e]) << 32 | (uint32_t)block_index(i0, 4 * j + e);
-            }
+            if (is && in_list(m)) put(v[e], 4 * j + e);
         }
     });
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -741,14 +801,14 @@ __global__ __launch_bounds__(kRowThreads) void tf_sample_draw_kernel(SampleArgs 
     ChunkStat mine_c{-INFINITY, 0, 0, 0};
     if (lane < a.chunks) mine_c = row_stats(a, row)[lane];
     RowInfo info = *row_info(a, row);
-    if (s.plain()) info.cut = 0;
+    if (s.plain()) info.cut = 0, info.wide = 0;
     // the list's length and each chunk's place in it; too long for LDS, or a chunk's for
     // its room: the row itself
     int list_upto = 0, count = 0;
     if (info.cut == 1) {
         list_upto = wave_scan(mine_c.listed);
         count = lane_value(list_upto, 63);
-        if (count > kList || __ballot(mine_c.listed > kChunkList)) info.cut = 2;
+        if (count > kList || __ballot(mine_c.listed > kChunkList)) info.cut = 2, info.wide = 0;
     }
     const int segments = (n + kSegment - 1) / kSegment;
     u64 my_seg = 0;
@@ -818,7 +878,8 @@ __global__ __launch_bounds__(kRowThreads) void tf_sample_draw_kernel(SampleArgs 
         each([&](uint32_t key, int i) {
             if (!cut.keeps(key, i)) return;
             const double we = w(key_logit(key));
-            if (we >= s.min_w) atomicAdd(&seg_sum[i / kSegment], row_units(we));
+            if (we >= s.min_w)
+                atomicAdd(&seg_sum[(i / kSegment) & (info.wide ? -kWide : ~0)], row_units(we));
         });
         __syncthreads();
     } else if (info.cut == 2) {
@@ -895,25 +956,39 @@ __global__ __launch_bounds__(kRowThreads) void tf_sample_draw_kernel(SampleArgs 
     u = u > 0.0 ? u : 0.0;  // NaN: 0
     const double target = u * total;
     // the first that passes the target (rounding may leave none: the last with a weight)
-    auto choose = [&](bool passes, bool any, int at) {
+    auto choose = [&](bool passes, int at, bool any, int last) {
         __syncthreads();
         if (tid == 0) answer = -1, total_w = ~0ull;
         __syncthreads();
         const u64 hits = __ballot(passes), has = __ballot(any);
         if (hits && lane == __builtin_ctzll(hits)) atomicMin(&total_w, (u64)at);
-        if (has && lane == 63 - __builtin_clzll(has)) atomicMax(&answer, at);
+        if (has && lane == 63 - __builtin_clzll(has)) atomicMax(&answer, last);
         __syncthreads();
         return total_w != ~0ull ? (int)total_w : max(answer, 0);
     };
-    const int seg = choose(seg_w > 0.0 && upto > target, seg_w > 0.0, tid);
+    const int seg = choose(seg_w > 0.0 && upto > target, tid, seg_w > 0.0, tid);
     if (seg == tid) seg_before = upto - seg_w;
-    const int i = seg * kSegment + tid;
-    const float l = i < n ? x[i] : -INFINITY;
-    __syncthreads();
-    const double before = seg_before, v = i < n ? weight_of(l, i) : 0.0;
-    double all;
-    upto = before + scan(v, all);
-    const int at = choose(v > 0.0 && upto > target, v > 0.0, i);
+    const int per = info.wide ? kWide : 1, i = seg * kSegment + per * tid;
+    double v[kWide], sum = 0.0, all;
+    float l[kWide];
+#pragma unroll
+    for (int e = 0; e < kWide; e++) l[e] = e < per && i + e < n ? x[i + e] : -INFINITY;
+#pragma unroll
+    for (int e = 0; e < kWide; e++) {
+        v[e] = e < per && i + e < n ? weight_of(l[e], i + e) : 0.0;
+        sum += v[e];
+    }
+    const double upto_i = scan(sum, all);
+    // falling from the lane's last: the first that passes, and the last with a weight
+    double run = seg_before + upto_i;
+    int pass_at = -1, last_at = -1;
+#pragma unroll
+    for (int e = kWide - 1; e >= 0; e--) {
+        if (v[e] > 0.0 && run > target) pass_at = i + e;
+        if (v[e] > 0.0) last_at = max(last_at, i + e);
+        run -= v[e];
+    }
+    const int at = choose(pass_at >= 0, pass_at, last_at >= 0, last_at);
     if (tid == 0) a.out[row] = at;
 }
 
