@@ -631,8 +631,8 @@ struct Select {
     u64 hist[256];
     u64 left;
     u64 few[64];  // elements that are ranked directly
-    int digit, count;
-    uint32_t least, most;
+    uint32_t many[256];  // elements of each digit
+    int digit, count, place;
 };
 
 // The largest digit d such that the total of digits >= d reaches s.left, which
@@ -710,60 +710,51 @@ __device__ Cut select_cut(Select& s, u64 goal, Each each, Value value) {
     return {prefix, (int)(~at & 0xffffffu)};
 }
 
-// The same for elements in LDS, whose keys lie close (one bin's): one pass over 256 equal
-// steps from the least key to the most leaves a handful, and a wave ranks up to 64 by
-// comparing each with all.
-template <class Each, class Value>
-__device__ Cut select_near(Select& s, u64 goal, Each each, Value value) {
+// The same for elements in LDS, of a few bins: step(key) of 0 .. 255, which rises as keys
+// fall.  One pass over the steps leaves a handful, and a wave ranks up to 64 by comparing
+// each with all.
+template <class Each, class Value, class Step>
+__device__ Cut select_near(Select& s, u64 goal, Each each, Value value, Step step) {
     const int tid = threadIdx.x, lane = tid & 63;
     if (goal < 1) goal = 1;
+    if (tid < 256) s.hist[tid] = 0, s.many[tid] = 0;
     __syncthreads();
-    if (tid == 0) s.count = 0, s.least = ~0u, s.most = 0, s.left = goal;
-    if (tid < 256) s.hist[tid] = 0;
-    __syncthreads();
-    uint32_t least = ~0u, most = 0;
-    int mine = 0;
     each([&](uint32_t key, int) {
-        least = min(least, key);
-        most = max(most, key);
-        mine++;
+        const int d = step(key);
+        atomicAdd(&s.hist[d], value(key));
+        atomicAdd(&s.many[d], 1u);
     });
-    // one atomic a wave: a wave's lanes on one address go one after the other
-    least = ~wave_max_u32(~least);
-    most = wave_max_u32(most);
-    mine = wave_sum(mine);
-    if (mine && lane == 0) {
-        atomicMin(&s.least, least);
-        atomicMax(&s.most, most);
-        atomicAdd(&s.count, mine);
+    __syncthreads();
+    if (tid < 64) {  // the first step at which the total reaches the goal
+        u64 h[4], sum = 0;
+        uint32_t m[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            sum += h[i] = s.hist[4 * lane + i];
+            m[i] = s.many[4 * lane + i];
+        }
+        const u64 upto = wave_scan(sum), over = __ballot(upto >= goal);
+        // none: the goal is past them all, to which rounding may have led: the last
+        const u64 has = __ballot(m[0] | m[1] | m[2] | m[3]);
+        const int who = over ? __builtin_ctzll(over) : has ? 63 - __builtin_clzll(has) : 0;
+        if (lane == who) {
+            u64 run = upto - sum;
+            int i = 0;
+            if (over)
+                while (i < 3 && run + h[i] < goal) run += h[i++];
+            else
+                for (i = 3; i > 0 && !m[i];) i--;
+            s.digit = 4 * lane + i;
+            s.left = over ? goal - run : ~0ull;
+            s.count = m[i];
+            s.place = 0;
+        }
     }
     __syncthreads();
-    int count = s.count;
-    uint32_t from = 0, span = ~0u;  // keys still in question: from .. from + span
-    if (count > 64) {
-        const uint32_t lowest = s.least;
-        const int shift = max(24 - __builtin_clz((s.most - lowest) | 1), 0);
-        each([&](uint32_t key, int) { atomicAdd(&s.hist[(key - lowest) >> shift], value(key)); });
-        __syncthreads();
-        if (tid < 64) pick_digit(s);
-        if (tid == 0) s.count = 0;
-        __syncthreads();
-        from = lowest + ((uint32_t)s.digit << shift);
-        span = (1u << shift) - 1;  // the end may lie past 2^32
-        mine = 0;
-        each([&](uint32_t key, int) { mine += key - from <= span; });
-        mine = wave_sum(mine);
-        if (mine && lane == 0) atomicAdd(&s.count, mine);
-        __syncthreads();
-        count = s.count;
-        if (count > 64) return select_cut(s, goal, each, value);
-    }
-    __syncthreads();
-    if (tid == 0) s.count = 0;
-    __syncthreads();
+    const int digit = s.digit, count = s.count;
+    if (count > 64) return select_cut(s, goal, each, value);
     each([&](uint32_t key, int index) {
-        if (key - from <= span)
-            s.few[atomicAdd(&s.count, 1)] = (u64)key << 32 | (uint32_t)~index;
+        if (step(key) == digit) s.few[atomicAdd(&s.place, 1)] = (u64)key << 32 | (uint32_t)~index;
     });
     __syncthreads();
     if (tid < 64) {
@@ -773,7 +764,6 @@ __device__ Cut select_near(Select& s, u64 goal, Each each, Value value) {
         for (int j = 0; j < count; j++) before += lane_value(me, j) > me ? lane_value(part, j) : 0;
         const u64 left = s.left;
         const u64 hit = __ballot(lane < count && before < left && before + part >= left);
-        // none: the goal is past them all, to which rounding may have led
         u64 last = ~0ull;
         if (!hit)
             for (int j = 0; j < count; j++) last = min(last, lane_value(me, j));
@@ -789,9 +779,9 @@ __global__ __launch_bounds__(kRowThreads) void tf_sample_draw_kernel(SampleArgs 
     u64* list = reinterpret_cast<u64*>(lds);                        // kList
     u64* seg_sum = list + kList;                                    // kMaxSegments
     Select& sel = *reinterpret_cast<Select*>(seg_sum + kMaxSegments);
-    __shared__ double wave_w[kRowWaves], table[32], seg_before;
+    __shared__ double wave_w[2][kRowWaves], table[32], seg_before;
     __shared__ u64 total_w;
-    __shared__ int answer;
+    __shared__ int first_at[2], last_at[2];
     const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const float* x = a.logits + (size_t)row * a.stride;
@@ -824,7 +814,8 @@ __global__ __launch_bounds__(kRowThreads) void tf_sample_draw_kernel(SampleArgs 
     const RowWeight w(table, s.temp, l_max);
     auto units = [&](uint32_t key) { return row_units(w(key_logit(key))); };
     auto one = [](uint32_t) { return (u64)1; };
-    if (tid == 0) answer = -1, total_w = 0;
+    if (tid == 0) total_w = 0;
+    if (tid < 2) first_at[tid] = INT32_MAX, last_at[tid] = -1;
     if (tid < segments) seg_sum[tid] = my_seg;
     __syncthreads();
 
@@ -836,13 +827,19 @@ __global__ __launch_bounds__(kRowThreads) void tf_sample_draw_kernel(SampleArgs 
             const u64* src = chunk_list(a, row, c);
             for (int i = lane; i < have; i += 64) list[to + i] = src[i];
         }
-        __syncthreads();
         const float base = bin_of(l_max, s.per_l);
         auto each = [&](auto f) {
             for (int i = tid; i < count; i += kRowThreads)
                 f((uint32_t)(list[i] >> 32), (int)(uint32_t)list[i]);
         };
         auto bin = [&](uint32_t key) { return bin_below(base, bin_of(key_logit(key), s.per_l)); };
+        // 256 steps over bins b0 .. b1
+        auto steps = [&](int b0, int b1) {
+            const float top = base - (float)(b0 - 1), per = 256.f / (float)(b1 - b0 + 1);
+            return [=](uint32_t key) {
+                return (int)fminf(fmaxf((top - key_logit(key) * s.per_l) * per, 0.f), 255.f);
+            };
+        };
         u64 kept_w = info.w_all;
         if (info.use_k) {
             auto in_k = [&](auto f) {
@@ -850,7 +847,8 @@ __global__ __launch_bounds__(kRowThreads) void tf_sample_draw_kernel(SampleArgs 
                     if (bin(key) == info.k_bin) f(key, i);
                 });
             };
-            cut = select_near(sel, (u64)(s.k - info.k_before), in_k, one);
+            cut = select_near(sel, (u64)(s.k - info.k_before), in_k, one,
+                              steps(info.k_bin, info.k_bin));
             if (s.use_p) {
                 u64 add = 0;
                 in_k([&](uint32_t key, int i) { add += cut.keeps(key, i) ? units(key) : 0; });
@@ -871,7 +869,7 @@ __global__ __launch_bounds__(kRowThreads) void tf_sample_draw_kernel(SampleArgs 
                         if (b >= info.lo && b <= info.hi && k_cut.keeps(key, i)) f(key, i);
                     });
                 },
-                units);
+                units, steps(info.lo, info.hi));
             cut.within(k_cut);
         }
         // what the list adds to each segment
@@ -914,17 +912,16 @@ __global__ __launch_bounds__(kRowThreads) void tf_sample_draw_kernel(SampleArgs 
         const double v = w(l);
         return v >= s.min_w ? v : 0.0;
     };
-    // inclusive running sum over the workgroup, and the sum
-    auto scan = [&](double v, double& all) {
+    // inclusive running sum over the workgroup, and the sum; each once, with its own LDS
+    auto scan = [&](int which, double v, double& all) {
         const double upto = wave_scan(v);
-        __syncthreads();
-        if (lane == 63) wave_w[wave] = upto;
+        if (lane == 63) wave_w[which][wave] = upto;
         __syncthreads();
         double ahead = 0.0;
         all = 0.0;
         for (int i = 0; i < kRowWaves; i++) {
-            if (i < wave) ahead += wave_w[i];
-            all += wave_w[i];
+            if (i < wave) ahead += wave_w[which][i];
+            all += wave_w[which][i];
         }
         return ahead + upto;
     };
@@ -951,22 +948,20 @@ __global__ __launch_bounds__(kRowThreads) void tf_sample_draw_kernel(SampleArgs 
             seg_w = (double)b * (1.0 / kRowUnit);
         }
     }
-    double total, upto = scan(seg_w, total);
+    double total;
+    const double upto = scan(0, seg_w, total);
     double u = (double)a.u[row];
     u = u > 0.0 ? u : 0.0;  // NaN: 0
     const double target = u * total;
     // the first that passes the target (rounding may leave none: the last with a weight)
-    auto choose = [&](bool passes, int at, bool any, int last) {
-        __syncthreads();
-        if (tid == 0) answer = -1, total_w = ~0ull;
-        __syncthreads();
+    auto choose = [&](int which, bool passes, int at, bool any, int last) {
         const u64 hits = __ballot(passes), has = __ballot(any);
-        if (hits && lane == __builtin_ctzll(hits)) atomicMin(&total_w, (u64)at);
-        if (has && lane == 63 - __builtin_clzll(has)) atomicMax(&answer, last);
+        if (hits && lane == __builtin_ctzll(hits)) atomicMin(&first_at[which], at);
+        if (has && lane == 63 - __builtin_clzll(has)) atomicMax(&last_at[which], last);
         __syncthreads();
-        return total_w != ~0ull ? (int)total_w : max(answer, 0);
+        return first_at[which] != INT32_MAX ? first_at[which] : max(last_at[which], 0);
     };
-    const int seg = choose(seg_w > 0.0 && upto > target, tid, seg_w > 0.0, tid);
+    const int seg = choose(0, seg_w > 0.0 && upto > target, tid, seg_w > 0.0, tid);
     if (seg == tid) seg_before = upto - seg_w;
     const int per = info.wide ? kWide : 1, i = seg * kSegment + per * tid;
     double v[kWide], sum = 0.0, all;
@@ -978,17 +973,17 @@ __global__ __launch_bounds__(kRowThreads) void tf_sample_draw_kernel(SampleArgs 
         v[e] = e < per && i + e < n ? weight_of(l[e], i + e) : 0.0;
         sum += v[e];
     }
-    const double upto_i = scan(sum, all);
+    const double upto_i = scan(1, sum, all);
     // falling from the lane's last: the first that passes, and the last with a weight
     double run = seg_before + upto_i;
-    int pass_at = -1, last_at = -1;
+    int pass = -1, last = -1;
 #pragma unroll
     for (int e = kWide - 1; e >= 0; e--) {
-        if (v[e] > 0.0 && run > target) pass_at = i + e;
-        if (v[e] > 0.0) last_at = max(last_at, i + e);
+        if (v[e] > 0.0 && run > target) pass = i + e;
+        if (v[e] > 0.0) last = max(last, i + e);
         run -= v[e];
     }
-    const int at = choose(pass_at >= 0, pass_at, last_at >= 0, last_at);
+    const int at = choose(1, pass >= 0, pass, last >= 0, last);
     if (tid == 0) a.out[row] = at;
 }
 
