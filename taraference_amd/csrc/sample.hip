@@ -781,7 +781,7 @@ __global__ __launch_bounds__(kRowThreads) void tf_sample_draw_kernel(SampleArgs 
     Select& sel = *reinterpret_cast<Select*>(seg_sum + kMaxSegments);
     __shared__ double wave_w[2][kRowWaves], table[32], seg_before;
     __shared__ u64 total_w;
-    __shared__ int first_at[2], last_at[2];
+    __shared__ int first_at[2], last_at[2], chunk_upto[kMaxChunks];
     const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const float* x = a.logits + (size_t)row * a.stride;
@@ -817,15 +817,17 @@ __global__ __launch_bounds__(kRowThreads) void tf_sample_draw_kernel(SampleArgs 
     if (tid == 0) total_w = 0;
     if (tid < 2) first_at[tid] = INT32_MAX, last_at[tid] = -1;
     if (tid < segments) seg_sum[tid] = my_seg;
+    if (tid < kMaxChunks) chunk_upto[tid] = list_upto;
     __syncthreads();
 
     Cut cut{0u, kMaxVocab};
     if (info.cut == 1) {
-        for (int c = wave; c < a.chunks; c += kRowWaves) {
-            const int have = __builtin_amdgcn_readlane(mine_c.listed, c);
-            const int to = __builtin_amdgcn_readlane(list_upto, c) - have;
-            const u64* src = chunk_list(a, row, c);
-            for (int i = lane; i < have; i += 64) list[to + i] = src[i];
+        for (int i = tid; i < count; i += kRowThreads) {
+            int c = 0;  // its chunk: as many end at or before i
+#pragma unroll
+            for (int b = kMaxChunks / 2; b; b >>= 1)
+                if (chunk_upto[c + b - 1] <= i) c += b;
+            list[i] = chunk_list(a, row, c)[i - (c ? chunk_upto[c - 1] : 0)];
         }
         const float base = bin_of(l_max, s.per_l);
         auto each = [&](auto f) {
