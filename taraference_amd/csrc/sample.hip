@@ -453,6 +453,16 @@ __global__ __launch_bounds__(kChunkThreads, 6) void tf_sample_gather_kernel(Samp
         return;
     }
     const float base = bin_of(l_max, s.per_l);
+    // min-p's bound on the product that places an element: one above m_keep is past it and
+    // one below m_drop is not, whatever the rounding of products, logarithm and sums
+    float m_keep = -INFINITY, m_drop = -INFINITY;
+    {
+        const float m_top = l_max * s.per_l;
+        const float depth = s.min_w > 0.0 ? -__log2f((float)s.min_w) * (0.69314718f * kPerZ)
+                                          : INFINITY;
+        const float margin = 0.02f + (fabsf(m_top) + depth) * 0x1p-21f;
+        if (margin < INFINITY) m_keep = m_top - depth + margin, m_drop = m_top - depth - margin;
+    }
     if (tid < 3) first[tid] = kBins - 1;
     if (tid == 0) place = 0;
     __syncthreads();  // the table
@@ -523,12 +533,9 @@ __global__ __launch_bounds__(kChunkThreads, 6) void tf_sample_gather_kernel(Samp
             info.cut = 1;
             info.w_before_lo = lo ? w_upto[lo - 1] : 0;
             auto in_bins = [&](int b0, int b1) { return n_upto[b1] - (b0 ? n_upto[b0 - 1] : 0); };
-            // the bins in which min-p's bound lies: its distance below the largest, in bins, to
-            // a bin and the rounding of the products that place an element
-            const float depth = s.min_w > 0.0 ? -__log2f((float)s.min_w) * (0.69314718f * kPerZ)
-                                              : INFINITY;
-            const int first_m = (int)fminf(fmaxf(ceilf(depth - 1.7f), 0.f), (float)kBins);
-            const bool m_first = depth + 1.7f < (float)lo;
+            // the bins that min-p's bound cuts
+            const int first_m = (int)fminf(fmaxf(base - floorf(m_keep), 0.f), (float)kBins);
+            const bool m_first = base - floorf(m_drop) < (float)lo;
             list_from = min(lo, first_m);
             // with top-k the list's length is known here; else the draw finds it too long
             const u64 listed = in_bins(list_from, hi) + (k_bin > hi ? in_bins(k_bin, k_bin) : 0);
@@ -548,15 +555,12 @@ __global__ __launch_bounds__(kChunkThreads, 6) void tf_sample_gather_kernel(Samp
     // the chunk's part of the list, and its weight before it
     // bins as bounds on the product that bin_of() rounds down: bin b holds base - b <= l
     // per_l < base - b + 1, the last one all below
-    // (min-p alone: what it may keep, a bin and the rounding of the products below it)
-    const bool min_p = lo == kBins && fabsf(base) < 1e5f, all = lo == kBins && !min_p;
-    const float sure = lo < kBins ? base - (float)(list_from - 1)
-                       : min_p    ? base - 2.f + __log2f((float)s.min_w) * (0.69314718f * kPerZ)
-                                  : -INFINITY;
+    const float sure = lo < kBins ? base - (float)(list_from - 1) : m_drop;
     const float listed = hi < kBins - 1 ? base - (float)hi : -INFINITY;
     const float k_from = k_bin < 0 ? INFINITY : k_bin < kBins - 1 ? base - (float)k_bin : -INFINITY;
     const float k_to = base - (float)(k_bin - 1);
     const float low = hi >= 0 ? fminf(listed, k_from) : sure;
+    const bool all = sure == -INFINITY;  // products may be NaN
     auto in_list = [&](float m) {
         return m < sure && ((hi >= 0 && m >= listed) || (m >= k_from && m < k_to));
     };

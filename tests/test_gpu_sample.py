@@ -200,3 +200,24 @@ def test_long_lists(gpu):
         us = np.full(4, u, np.float32)
         for a in ({"k": [1234] * 4}, {"p": [0.61] * 4}, {"k": [1999] * 4, "p": [0.37] * 4}):
             assert np.array_equal(draw(gpu, x, us, **a), want(x, us, **a)), (u, a)
+
+
+@pytest.mark.parametrize("body,t", [(2.0, 1.0), (3.0, 4.0), (300.0, 150.0)])
+def test_min_p_beside_the_other_cuts(gpu, body, t):
+    """min-p's bound in, just before and just behind the bins that top-k or top-p cuts, on
+    rows far from zero too (where a bin's bounds round)."""
+    rng = np.random.default_rng(14)
+    n = 30000
+    x = (body * rng.standard_normal((5, n))).astype(np.float32)
+    x[1] += 1e4
+    x[2] -= 3e4
+    x[3] += 2e5
+    w = np.exp((x.astype(np.float64) - x.max(1, keepdims=True)) / t)
+    for m in (0.5, 0.05, 1e-3):
+        for near in (0.6, 0.98, 1.0, 1.02, 1.7):
+            above = w >= m * near
+            k, p = above.sum(1), np.minimum((w * above).sum(1) / w.sum(1), 0.9999)
+            for a in ({"k": k}, {"p": p}, {"k": k + 3, "p": p * 0.999}):
+                a = {**a, "t": [t] * 5, "m": [m] * 5}
+                us = rng.random(5).astype(np.float32)
+                assert np.array_equal(draw(gpu, x, us, **a), want(x, us, **a)), (m, near, a)
