@@ -52,6 +52,8 @@ typedef unsigned long long u64;
 
 // 512 bins of 1/16: one row's first launch 11 us instead of 7, by LDS atomics and scans.
 constexpr int kBins = 256;          // of 1/8 of z: 32 below a chunk's largest, the last open
+constexpr int kMaxFine = 16;        // finer ones, by powers of two, where a chunk's spread is less
+constexpr float kNoWeight = 5560.f; // bins below the largest from which exp2_neg() gives 0
 constexpr float kPerZ = 8.f;
 constexpr int kList = 8192;         // elements of a row's list, and
 constexpr int kChunkList = 2048;    // of a chunk's part of it
@@ -100,13 +102,14 @@ struct RowInfo {
     u64 w_before_k, w_before_lo, w_all;  // weights in bins before k_bin, before lo, in all
     int cut;                    // 0: no cut, kept is what min-p keeps; 1: the list; 2: the row itself
     int use_k;                  // top-k cuts something
+    int fine;                   // the row's bins are 2^-fine of the widest
     int wide;                   // segments' sums are of kWide, in the first one's place
 };
 struct ChunkStat {
     float top;    // the largest logit
     int index;    // its lowest index (T <= 0 only)
     int listed;   // elements of its list
-    int pad;
+    int fine;     // its bins are 2^-fine of the widest
 };
 __device__ __forceinline__ RowInfo* row_info(const SampleArgs& a, int row) {
     return reinterpret_cast<RowInfo*>(a.ws + row * a.row_bytes);
@@ -338,7 +341,7 @@ __global__ __launch_bounds__(kChunkThreads, 6) void tf_sample_stats_kernel(Sampl
     __shared__ uint32_t count[4][kBins + 16];
     __shared__ double table[32];
     __shared__ u64 totals[kParts][kChunkWaves];
-    __shared__ float part[kChunkWaves];
+    __shared__ float part[kChunkWaves], part_low[kChunkWaves];
     __shared__ int first;
     const int row = blockIdx.x / a.chunks, c = blockIdx.x - row * a.chunks;
     const int tid = threadIdx.x, lane = tid & 63;
@@ -374,6 +377,23 @@ __global__ __launch_bounds__(kChunkThreads, 6) void tf_sample_stats_kernel(Sampl
     }
     if (!s.filtered() && !s.plain()) return;
     const RowWeight w(table, s.temp, top);
+    int fine = 0;
+    if (s.filtered() && !empty && !s.bad) {
+        // the finest bins that hold all elements within 32 of the largest
+        float low = top;
+        const float far = top - 254.f / kPerZ * s.temp;
+#pragma unroll
+        for (int e = 0; e < 16; e++) low = fminf(low, v[e] > far ? v[e] : top);
+        low = -tf_wave_max(-low);
+        if (lane == 0) part_low[wave] = low;
+        __syncthreads();
+        for (int i = 0; i < kChunkWaves; i++) low = fminf(low, part_low[i]);
+        const float spread = fmaxf((top - low) * s.per_l, 1e-6f);
+        const float at = fmaxf(fabsf(top) * s.per_l, 1e-6f);
+        fine = (int)floorf(fminf(__log2f(252.f / spread), __log2f(0x1p21f / at)));
+        fine = max(0, min(fine, kMaxFine));
+        if (tid == 0) stat->fine = fine;
+    }
     if (s.plain()) {
         double sum = 0.0;
         if (!empty)
@@ -388,13 +408,15 @@ __global__ __launch_bounds__(kChunkThreads, 6) void tf_sample_stats_kernel(Sampl
         return;
     }
     if (!empty && !s.bad) {
-        const float base = bin_of(top, s.per_l);
+        const float per_l = ldexpf(s.per_l, fine), base = bin_of(top, per_l);
+        const float far = ldexpf(kNoWeight, fine);
         const int copy = 2 * (wave / (kChunkWaves / kParts)) + (lane & 1);
         each_four(v, [&](int) {
 #pragma unroll
-            for (int e = 0; e < 4; e++) {  // -inf and NaN add nothing
-                const int bin = bin_below(base, bin_of(v[e], s.per_l));
-                if (s.use_k) atomicAdd(&count[lane & 3][bin], v[e] > -INFINITY ? 1u : 0u);
+            for (int e = 0; e < 4; e++) {  // -inf, NaN and what has no weight add nothing
+                const float b = bin_of(v[e], per_l);
+                const int bin = bin_below(base, b);
+                if (s.use_k) atomicAdd(&count[lane & 3][bin], base - b <= far ? 1u : 0u);
                 if (s.use_p) atomicAdd(&weight[copy][bin], chunk_units(w(v[e])));
             }
         });
@@ -437,9 +459,10 @@ __global__ __launch_bounds__(kChunkThreads, 6) void tf_sample_gather_kernel(Samp
     const int i0 = c * kBlock, end = min(i0 + kBlock, a.n);
     float v[16];
     load_block(x, i0, end, v);
-    const Settings s = settings(a, row);
+    Settings s = settings(a, row);
     float mine_top = -INFINITY;
-    if (lane < a.chunks) mine_top = row_stats(a, row)[lane].top;
+    int mine_fine = kMaxFine;
+    if (lane < a.chunks) mine_top = row_stats(a, row)[lane].top, mine_fine = row_stats(a, row)[lane].fine;
     // the workgroup's first half adds up the histograms' counts, the second their weights
     const int half = wave / (kChunkWaves / 2), bin = tid % kBins;
     fill_exp2(table);
@@ -452,27 +475,37 @@ __global__ __launch_bounds__(kChunkThreads, 6) void tf_sample_gather_kernel(Samp
         if (c == 0 && tid == 0) *row_info(a, row) = info;
         return;
     }
+    __syncthreads();  // the table
+    const RowWeight w(table, s.temp, l_max);
+    // of chunk `lane`: its weights' scale, its bins' size and its largest's
+    const double lane_f = mine_top > -INFINITY ? w(mine_top) * (kRowUnit / kChunkUnit) : 0.0;
+    const bool any = lane_f > 0.0;
+    info.fine = s.filtered() ? kMaxFine - (int)wave_max_u32(any ? kMaxFine - mine_fine : 0) : 0;
+    const float lane_base = bin_of(mine_top, ldexpf(s.per_l, mine_fine));
+    const float lane_step = ldexpf(1.f, mine_fine - info.fine);
+    s.per_l = ldexpf(s.per_l, info.fine);
     const float base = bin_of(l_max, s.per_l);
     // min-p's bound on the product that places an element: one above m_keep is past it and
     // one below m_drop is not, whatever the rounding of products, logarithm and sums
     float m_keep = -INFINITY, m_drop = -INFINITY;
     {
         const float m_top = l_max * s.per_l;
-        const float depth = s.min_w > 0.0 ? -__log2f((float)s.min_w) * (0.69314718f * kPerZ)
+        const float depth = s.min_w > 0.0 ? -__log2f((float)s.min_w) * ldexpf(0.69314718f * kPerZ, info.fine)
                                           : INFINITY;
         const float margin = 0.02f + (fabsf(m_top) + depth) * 0x1p-21f;
         if (margin < INFINITY) m_keep = m_top - depth + margin, m_drop = m_top - depth - margin;
     }
     if (tid < 3) first[tid] = kBins - 1;
     if (tid == 0) place = 0;
-    __syncthreads();  // the table
-    const RowWeight w(table, s.temp, l_max);
+    __syncthreads();
     int lo = kBins, hi = -1, k_bin = -1;  // min-p alone: no cut by bins
     int list_from = kBins;
-    // of chunk `lane`: how far its bins lie below the row's, and its weights' scale
-    const bool any = mine_top > -INFINITY;
-    const int lane_shift = any ? bin_below(base, bin_of(mine_top, s.per_l)) : kBins;
-    const double lane_f = any ? w(mine_top) * (kRowUnit / kChunkUnit) : 0.0;
+    // a chunk's bin with which those up to a row's bin end (< 0: none)
+    auto chunk_bin = [&](int cc, int bin) {
+        if (bin == kBins - 1) return bin;
+        const float at = lane_value(lane_base, cc) - (base - (float)bin) * lane_value(lane_step, cc);
+        return (int)fminf(fmaxf(at, -1.f), (float)(kBins - 2));
+    };
     if (s.filtered()) {
         // the row's total up to a bin: each chunk's up to the bin that lies as far below its
         // own largest, weights scaled alike; the last bin has all there is.  Sums of rising
@@ -486,15 +519,14 @@ __global__ __launch_bounds__(kChunkThreads, 6) void tf_sample_gather_kernel(Samp
 #pragma unroll
                 for (int i = 0; i < kAtOnce; i++) {  // all loads at once
                     const int cc = min(c0 + i, a.chunks - 1);
-                    const int shift = __builtin_amdgcn_readlane(lane_shift, cc);
-                    const int from = bin == kBins - 1 ? bin : bin - shift;
+                    const int from = chunk_bin(cc, bin);
                     got[i] = (of + (size_t)cc * kChunkWords)[(uint32_t)max(from, 0)];
                     if (from < 0) got[i] = 0.0;
                 }
 #pragma unroll
                 for (int i = 0; i < kAtOnce; i++)
                     if (c0 + i < a.chunks)
-                        total += got[i] * (half ? lane_value(lane_f, c0 + i) : 1.0);
+                        total += got[i] * lane_value(half ? lane_f : any ? 1.0 : 0.0, c0 + i);
             }
         }
         u64* upto_of = half ? w_upto : n_upto;
@@ -556,8 +588,9 @@ __global__ __launch_bounds__(kChunkThreads, 6) void tf_sample_gather_kernel(Samp
     // bins as bounds on the product that bin_of() rounds down: bin b holds base - b <= l
     // per_l < base - b + 1, the last one all below
     const float sure = lo < kBins ? base - (float)(list_from - 1) : m_drop;
-    const float listed = hi < kBins - 1 ? base - (float)hi : -INFINITY;
-    const float k_from = k_bin < 0 ? INFINITY : k_bin < kBins - 1 ? base - (float)k_bin : -INFINITY;
+    const float no_weight = base - ldexpf(kNoWeight, info.fine);
+    const float listed = hi < kBins - 1 ? base - (float)hi : no_weight;
+    const float k_from = k_bin < 0 ? INFINITY : k_bin < kBins - 1 ? base - (float)k_bin : no_weight;
     const float k_to = base - (float)(k_bin - 1);
     const float low = hi >= 0 ? fminf(listed, k_from) : sure;
     const bool all = sure == -INFINITY;  // products may be NaN
@@ -580,7 +613,7 @@ __global__ __launch_bounds__(kChunkThreads, 6) void tf_sample_gather_kernel(Samp
         }
         if (tid < kParts) {  // a part's total is what it adds to those before it
             const double* of = chunk_totals(a, row, c) + kBins;
-            const int from = list_from - 1 - __builtin_amdgcn_readlane(lane_shift, c);
+            const int from = list_from > 0 ? chunk_bin(c, list_from - 1) : -1;
             double w_q = 0.0;
             if (from >= 0)
                 w_q = (of[tid * kBins + from] - (tid ? of[(tid - 1) * kBins + from] : 0.0)) *
@@ -803,7 +836,7 @@ __global__ __launch_bounds__(kRowThreads) void tf_sample_draw_kernel(SampleArgs 
     const float* x = a.logits + (size_t)row * a.stride;
     const int n = a.n;
     // everything that the workspace may hold of the row, at once
-    const Settings s = settings(a, row);
+    Settings s = settings(a, row);
     ChunkStat mine_c{-INFINITY, 0, 0, 0};
     if (lane < a.chunks) mine_c = row_stats(a, row)[lane];
     RowInfo info = *row_info(a, row);
@@ -845,6 +878,7 @@ __global__ __launch_bounds__(kRowThreads) void tf_sample_draw_kernel(SampleArgs 
                 if (chunk_upto[c + b - 1] <= i) c += b;
             list[i] = chunk_list(a, row, c)[i - (c ? chunk_upto[c - 1] : 0)];
         }
+        s.per_l = ldexpf(s.per_l, info.fine);
         const float base = bin_of(l_max, s.per_l);
         auto each = [&](auto f) {
             for (int i = tid; i < count; i += kRowThreads)

@@ -221,3 +221,28 @@ def test_min_p_beside_the_other_cuts(gpu, body, t):
                 a = {**a, "t": [t] * 5, "m": [m] * 5}
                 us = rng.random(5).astype(np.float32)
                 assert np.array_equal(draw(gpu, x, us, **a), want(x, us, **a)), (m, near, a)
+
+
+def test_chunks_of_many_spreads(gpu):
+    """Parts of a row that are flat, wide, far below the rest, masked by the lowest value or
+    empty, in one row."""
+    rng = np.random.default_rng(15)
+    n = 8192 * 7 + 100
+    x = rng.standard_normal((8, n)).astype(np.float32)
+    cut = np.arange(n) // 8192
+    for i in range(8):
+        for c in range(8):
+            at, kind = cut == c, rng.integers(0, 6)
+            x[i, at] *= np.float32([1e-4, 0.02, 1, 3, 40, 0][kind])
+            x[i, at] += np.float32(rng.choice([0, -0.5, -20, -400]) if i % 2 else 0)
+    x[2, cut == 3] = -np.inf
+    x[3, cut == 1] = np.finfo(np.float32).min
+    x[4, 15:] = np.finfo(np.float32).min
+    x[5, ::3] = np.finfo(np.float32).min
+    x[6] += 5e3
+    for t in (0.8, 30.0):
+        for a in ({"p": [0.3] * 8}, {"p": [0.97] * 8}, {"k": [40] * 8}, {"k": [30000] * 8},
+                  {"k": [9000] * 8, "p": [0.8] * 8}, {"k": [40] * 8, "p": [0.9] * 8, "m": [0.02] * 8}):
+            us = rng.random(8).astype(np.float32)
+            a = {**a, "t": [t] * 8}
+            assert np.array_equal(draw(gpu, x, us, **a), want(x, us, **a)), a
