@@ -32,7 +32,7 @@
 // Without top-k, top-p and min-p the second launch is left out.  A row whose
 // cut lies among more elements than the list holds (near-equal logits by the
 // ten thousand), or whose logits the bins cannot hold (an infinite one, T below
-// 1e-6), is selected by radix passes over the row itself in the third launch:
+// 1e-37), is selected by radix passes over the row itself in the third launch:
 // the same cut, found by one workgroup.
 //
 // One row of 151936 with all filters: 7.8 + 7.8 + 4.6 us, without filters 5.5 + 4.6;
@@ -52,7 +52,8 @@ typedef unsigned long long u64;
 
 // 512 bins of 1/16: one row's first launch 11 us instead of 7, by LDS atomics and scans.
 constexpr int kBins = 256;          // of 1/8 of z: 32 below a chunk's largest, the last open
-constexpr int kMaxFine = 16;        // finer ones, by powers of two, where a chunk's spread is less
+constexpr int kMaxFine = 16;        // finer ones, by powers of two, where a chunk's spread is less,
+constexpr int kMinFine = -240;      // and wider where their numbers would pass 2^21
 constexpr float kNoWeight = 5560.f; // bins below the largest from which exp2_neg() gives 0
 constexpr float kPerZ = 8.f;
 constexpr int kList = 8192;         // elements of a row's list, and
@@ -165,11 +166,11 @@ __device__ __forceinline__ Settings settings(const SampleArgs& a, int row) {
     const float m = uni(at(a.min_p, 0.f));
     s.min_w = m > 0.f ? fmin((double)m, 1.0) : 0.0;
     s.per_l = uni(kPerZ / s.temp);
-    s.bad = !(s.temp >= 1e-6f);
+    s.bad = !(s.temp >= 1e-37f);
     return s;
 }
-// Whether the bins can hold a row with this largest logit: their numbers are exact
-// floats up to 2^23.
+// Whether the bins can hold a row with this largest logit: their numbers are to be exact
+// floats.
 __device__ __forceinline__ bool no_bins(const Settings& s, float l_max) {
     return s.bad || !(fabsf(l_max) * s.per_l < 0x1p22f);
 }
@@ -389,9 +390,9 @@ __global__ __launch_bounds__(kChunkThreads, 6) void tf_sample_stats_kernel(Sampl
         __syncthreads();
         for (int i = 0; i < kChunkWaves; i++) low = fminf(low, part_low[i]);
         const float spread = fmaxf((top - low) * s.per_l, 1e-6f);
-        const float at = fmaxf(fabsf(top) * s.per_l, 1e-6f);
-        fine = (int)floorf(fminf(__log2f(252.f / spread), __log2f(0x1p21f / at)));
-        fine = max(0, min(fine, kMaxFine));
+        const float at = 21.f - __log2f(fabsf(top)) - __log2f(s.per_l);
+        fine = (int)floorf(fminf(__log2f(252.f / spread), fmaxf(at, (float)kMinFine)));
+        fine = max(kMinFine, min(fine, kMaxFine));
         if (tid == 0) stat->fine = fine;
     }
     if (s.plain()) {
@@ -409,7 +410,7 @@ __global__ __launch_bounds__(kChunkThreads, 6) void tf_sample_stats_kernel(Sampl
     }
     if (!empty && !s.bad) {
         const float per_l = ldexpf(s.per_l, fine), base = bin_of(top, per_l);
-        const float far = ldexpf(kNoWeight, fine);
+        const float far = 1.f + ldexpf(kNoWeight, fine);
         const int copy = 2 * (wave / (kChunkWaves / kParts)) + (lane & 1);
         each_four(v, [&](int) {
 #pragma unroll
@@ -470,11 +471,6 @@ __global__ __launch_bounds__(kChunkThreads, 6) void tf_sample_gather_kernel(Samp
     const float l_max = tf_wave_max(mine_top);
     if (!(l_max > -INFINITY)) return;
     RowInfo info{};
-    if (s.filtered() && no_bins(s, l_max)) {
-        info.cut = 2;
-        if (c == 0 && tid == 0) *row_info(a, row) = info;
-        return;
-    }
     __syncthreads();  // the table
     const RowWeight w(table, s.temp, l_max);
     // of chunk `lane`: its weights' scale, its bins' size and its largest's
@@ -484,6 +480,11 @@ __global__ __launch_bounds__(kChunkThreads, 6) void tf_sample_gather_kernel(Samp
     const float lane_base = bin_of(mine_top, ldexpf(s.per_l, mine_fine));
     const float lane_step = ldexpf(1.f, mine_fine - info.fine);
     s.per_l = ldexpf(s.per_l, info.fine);
+    if (s.filtered() && no_bins(s, l_max)) {
+        info.cut = 2;
+        if (c == 0 && tid == 0) *row_info(a, row) = info;
+        return;
+    }
     const float base = bin_of(l_max, s.per_l);
     // min-p's bound on the product that places an element: one above m_keep is past it and
     // one below m_drop is not, whatever the rounding of products, logarithm and sums
@@ -588,7 +589,7 @@ __global__ __launch_bounds__(kChunkThreads, 6) void tf_sample_gather_kernel(Samp
     // bins as bounds on the product that bin_of() rounds down: bin b holds base - b <= l
     // per_l < base - b + 1, the last one all below
     const float sure = lo < kBins ? base - (float)(list_from - 1) : m_drop;
-    const float no_weight = base - ldexpf(kNoWeight, info.fine);
+    const float no_weight = base - 1.f - ldexpf(kNoWeight, info.fine);
     const float listed = hi < kBins - 1 ? base - (float)hi : no_weight;
     const float k_from = k_bin < 0 ? INFINITY : k_bin < kBins - 1 ? base - (float)k_bin : no_weight;
     const float k_to = base - (float)(k_bin - 1);

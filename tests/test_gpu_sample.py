@@ -240,7 +240,7 @@ def test_chunks_of_many_spreads(gpu):
     x[4, 15:] = np.finfo(np.float32).min
     x[5, ::3] = np.finfo(np.float32).min
     x[6] += 5e3
-    for t in (0.8, 30.0):
+    for t in (0.8, 30.0, 3e-5, 1e-9, 1e-36):
         for a in ({"p": [0.3] * 8}, {"p": [0.97] * 8}, {"k": [40] * 8}, {"k": [30000] * 8},
                   {"k": [9000] * 8, "p": [0.8] * 8}, {"k": [40] * 8, "p": [0.9] * 8, "m": [0.02] * 8}):
             us = rng.random(8).astype(np.float32)
