@@ -683,6 +683,7 @@ struct Select {
     u64 few[64];  // elements that are ranked directly
     uint32_t many[256];  // elements of each digit
     int digit, count, place;
+    uint32_t least, most;
 };
 
 // The largest digit d such that the total of digits >= d reaches s.left, which
@@ -724,14 +725,29 @@ __device__ Cut select_cut(Select& s, u64 goal, Each each, Value value) {
         __syncthreads();
         return s.digit;
     };
-    if (tid == 0) s.left = goal > 0 ? goal : 1;
-    uint32_t prefix = 0;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        const uint32_t mask = shift == 24 ? 0u : ~0u << (shift + 8);
-        prefix |= (uint32_t)pass([&](uint32_t key, int) {
-                      return (key & mask) == prefix ? (int)(key >> shift & 255) : -1;
-                  })
-                  << shift;
+    // all alike (a row of zeros): no passes over the key
+    __syncthreads();
+    if (tid == 0) s.left = goal > 0 ? goal : 1, s.least = ~0u, s.most = 0;
+    __syncthreads();
+    uint32_t least = ~0u, most = 0;
+    each([&](uint32_t key, int) { least = min(least, key), most = max(most, key); });
+    least = ~wave_max_u32(~least);
+    most = wave_max_u32(most);
+    if ((tid & 63) == 0) {
+        atomicMin(&s.least, least);
+        atomicMax(&s.most, most);
+    }
+    __syncthreads();
+    uint32_t prefix = s.least;
+    if (s.least != s.most) {
+        prefix = 0;
+        for (int shift = 24; shift >= 0; shift -= 8) {
+            const uint32_t mask = shift == 24 ? 0u : ~0u << (shift + 8);
+            prefix |= (uint32_t)pass([&](uint32_t key, int) {
+                          return (key & mask) == prefix ? (int)(key >> shift & 255) : -1;
+                      })
+                      << shift;
+        }
     }
     // equal elements share the total: how many of them, and which index is the last
     const u64 each_value = value(prefix), left = s.left;
@@ -747,15 +763,27 @@ __device__ Cut select_cut(Select& s, u64 goal, Each each, Value value) {
     if (need >= s.hist[0]) return {prefix, kMaxVocab};
     __syncthreads();
     // the need-th lowest index: digits of its complement, so that falling order is rising
-    if (tid == 0) s.left = need * each_value;
+    if (tid == 0) s.left = need;
     uint32_t at = 0;
     for (int shift = 16; shift >= 0; shift -= 8) {
         const uint32_t mask = ~0u << (shift + 8) & 0xffffffu;
-        at |= (uint32_t)pass([&](uint32_t key, int index) {
-                  const uint32_t r = ~(uint32_t)index & 0xffffffu;
-                  return key == prefix && (r & mask) == at ? (int)(r >> shift & 255) : -1;
-              })
-              << shift;
+        __syncthreads();
+        if (tid < 256) s.hist[tid] = 0;
+        __syncthreads();
+        each([&](uint32_t key, int index) {
+            const uint32_t r = ~(uint32_t)index & 0xffffffu;
+            if (key != prefix || (r & mask) != at) return;
+            // neighbours share their digits: one of them adds for all
+            const int d = r >> shift & 255;
+            const u64 here = __ballot(true);
+            const bool alike = __ballot(d == __builtin_amdgcn_readfirstlane(d)) == here;
+            if (!alike || (tid & 63) == __builtin_ctzll(here))
+                atomicAdd(&s.hist[d], alike ? (u64)__popcll(here) : 1);
+        });
+        __syncthreads();
+        if (tid < 64) pick_digit(s);
+        __syncthreads();
+        at |= (uint32_t)s.digit << shift;
     }
     return {prefix, (int)(~at & 0xffffffu)};
 }
