@@ -537,8 +537,8 @@ int tf_flash_decode_kv8_n_split(int n_kv, int head_dim, int max_seq);
  * top_k <= 0 or >= n_vocab, top_p >= 1 and min_p <= 0 (and NaN) are off,
  * top_p <= 0 keeps one token, min_p > 1 counts as 1; temperature <= 0 (or NaN)
  * takes the largest logit, lowest index first.  u: a number in [0, 1) a row.
- * NaN and -inf are never drawn, +inf before all else; a row with nothing to
- * draw gives 0.  ws (16-byte aligned) holds tf_sample_ws_bytes(n_rows,
+ * NaN, -inf and weights below 2^-1000 are never drawn, +inf before all else; a
+ * row with nothing to draw gives 0.  ws (16-byte aligned) holds tf_sample_ws_bytes(n_rows,
  * n_vocab) bytes, which calls that run at the same time do not share. */
 int tf_sample(const float *logits, int n_rows, int n_vocab, int row_stride,
               const float *temperature, const int *top_k, const float *top_p,

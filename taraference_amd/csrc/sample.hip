@@ -29,18 +29,19 @@
 //      from the elements;
 //   3. draw: a workgroup a row takes the cuts from the list, finds the segments in
 //      which the running sum passes u, and walks those.
-// Without top-k, top-p and min-p the second launch is left out.  A row whose
-// cut lies among more elements than the list holds (near-equal logits by the
-// ten thousand), or whose logits the bins cannot hold (an infinite one, T below
-// 1e-37), is selected by radix passes over the row itself in the third launch:
-// the same cut, found by one workgroup.
+// Without top-k, top-p and min-p the second launch is left out.  A row whose cut lies
+// among more elements than the list holds (equal logits by the thousand), or whose logits
+// the bins cannot hold (an infinite one, T below 1e-37), is selected by radix passes over
+// the row itself in the third launch: the same cut, found by one workgroup (151936 equal
+// logits with top-p 312 us).  Bins of the row's own size keep others from there: logits
+// within 0.1 of each other, or T = 3, take the time of any row.
 //
-// One row of 151936 with all filters: 7.8 + 7.8 + 4.6 us, without filters 5.5 + 4.6;
-// bound by chains of loads and barriers (19 workgroups, then one).  64 rows with top-p:
-// 21.5 + 19.8 + 14.7 us.  There the first launch's 39 MB and largest take 13 of its us
-// and the exponentials 8 (they issue alongside: 60 VALU instructions for an element's
-// bin and weight in all); the atomics cost 1.  1216 workgroups run in two rounds of
-// three a CU: more a CU would spill registers, and cost 2 us.
+// One row of 151936 with all filters: 9 + 8 + 4.5 us, without filters 5.6 + 4.5; bound by
+// chains of loads and barriers (19 workgroups, then one).  64 rows with top-p: 23.2 + 19.9
+// + 14.7 us.  There the first launch has its VALU busy for 16 us (64 instructions for an
+// element's bin and weight); without exponentials it took 6.5 less, without the atomics 1.
+// 1216 workgroups run in two rounds of three a CU: more a CU would spill registers, and
+// cost 2 us.
 #include <math.h>
 
 #include "tf_common.hpp"
