@@ -20,7 +20,7 @@
 // named by its last element, and no row is sorted.  Three launches, rows cut
 // into chunks so that one row has the loads of many CUs:
 //   1. stats: a chunk's largest logit, and a histogram of counts (top-k) and
-//      weights (top-p) over bins of 1/8 of z below it (no filter: its sum of
+//      weights (top-p) over bins of 1/8 of z or less below it (no filter: its sum of
 //      weights);
 //   2. gather: each chunk's workgroup adds the row's histograms, finds the bins
 //      in which the cuts of top-k, top-p and min-p lie, and lists its elements of
