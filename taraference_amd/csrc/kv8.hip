@@ -429,17 +429,20 @@ __global__ __launch_bounds__(64 * TfKv8<HD>::W) void tf_flash_kv8_kernel(
         if (__ballot(tm > m) | __ballot(top >= vtop)) {
             tm = fmaxf(tm, __shfl_xor(tm, 16));
             tm = fmaxf(tm, __shfl_xor(tm, 32));
-            top = fmaxf(vtop, tf_wave_max(top));
+            top = tf_wave_max(top);
             const float m_new = fmaxf(m, tm);
             const float alpha = __expf(m - m_new);
-            // the power of two that takes scales up to `top` below 2^15
-            int fe = 141 - (int)(__float_as_uint(top) >> 23);
-            fe = fe > 126 ? 126 : fe < -126 ? -126 : fe;
-            const float f = __uint_as_float((uint32_t)(fe + 127) << 23);
-            // the first factor is whatever O = 0 takes
-            const float re = alpha * (vtop > 0.f ? f / vf : 1.f);
-            vf = f;
-            vtop = fe <= -113 ? INFINITY : __uint_as_float((uint32_t)(142 - fe) << 23);
+            float re = alpha;
+            if (top >= vtop) {  // wave-uniform; a larger maximum alone leaves the factor
+                // the power of two that takes scales up to `top` below 2^15
+                int fe = 141 - (int)(__float_as_uint(top) >> 23);
+                fe = fe > 126 ? 126 : fe < -126 ? -126 : fe;
+                const float f = __uint_as_float((uint32_t)(fe + 127) << 23);
+                // the first factor is whatever O = 0 takes
+                re *= vtop > 0.f ? f / vf : 1.f;
+                vf = f;
+                vtop = fe <= -113 ? INFINITY : __uint_as_float((uint32_t)(142 - fe) << 23);
+            }
             m = m_new;
             l *= alpha;
 #pragma unroll

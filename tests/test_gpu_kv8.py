@@ -236,3 +236,21 @@ def test_attention_of_scales_at_any_word(gpu):
         call("tf_flash_decode_kv8", P(dev(q)), P(dev(k8)), P(dkd) + 4, P(dev(v8)), P(dvd) + 4,
              P(part), P(out), None, None, h, kv, hd, seq - 1, None, n_split, 0.125, S())
         check(host(out).reshape(h, hd), q, ref.q8_values(k8, kd), ref.q8_values(v8, vd), kv, 0.125)
+
+
+@pytest.mark.parametrize("h,kv,hd", [(16, 2, 128), (14, 2, 64), (16, 1, 256), (3, 3, 128)])
+@pytest.mark.parametrize("seq,n_split", [(2000, 1), (20000, 1), (20000, 3)])
+def test_attention_whose_maximum_keeps_rising(gpu, h, kv, hd, seq, n_split):
+    """Scores that grow along the sequence: every tile of a long split renews the maximum.
+    (h == kv: one query head beside fifteen columns without one.)"""
+    rng = np.random.default_rng(seq + hd)
+    q = rng.standard_normal((h, hd)).astype(np.float32)
+    scale = 1 / np.sqrt(hd)
+    x = 0.2 * rng.standard_normal((seq, kv, hd))
+    for j in range(kv):  # along the group's mean query, up to a score of 8
+        m = q[j * (h // kv):(j + 1) * (h // kv)].mean(0)
+        x[:, j] += np.linspace(0, 8, seq)[:, None] * m / (m @ m) / scale
+    k8, kd = ref.q8_rows(x.reshape(seq, -1).astype(np.float32))
+    v8, vd = cache(rng, seq, kv * hd)
+    got = attend(q, dev(k8), dev(kd), dev(v8), dev(vd), kv, seq - 1, n_split, scale)[0]
+    check(got, q, ref.q8_values(k8, kd), ref.q8_values(v8, vd), kv, scale)
