@@ -515,7 +515,8 @@ int tf_kv8_read(const int8_t *k8, const float *kd, const int8_t *v8,
  * gives zeros), and with q8/d8 the Q8 of its output.  head_dim 64, 128 or
  * 256, n_head/n_kv <= 16, 1 <= n_split <= 1024; partial holds n_head *
  * n_split * (2 + head_dim) floats (not NULL, and not written, with one split).
- * q, k8 and v8 are 16-byte aligned, kd and vd too unless head_dim is 64. */
+ * q, k8 and v8 are 16-byte aligned, kd and vd too unless head_dim is 64.  A
+ * query that is infinite or NaN gives NaN in its own head alone. */
 int tf_flash_decode_kv8(const float *q, const int8_t *k8, const float *kd,
                         const int8_t *v8, const float *vd, float *partial,
                         float *out, int8_t *q8, float *d8, int n_head, int n_kv,

@@ -135,7 +135,7 @@ __global__ __launch_bounds__(256) void tf_kv8_read_kernel(const int8_t* __restri
 // % 16, g = l / 16: A[n][8g ..], B[8g ..][n], C[4g + r][n]):
 //   K Q^T  one k step is one scale group: A = 8 bytes of token n (or 16 + n), as
 //          f16 (exact), B = 8 dims of head n in two f16 parts after a power of
-//          two (2^-22 of the largest); the sums of a group are f32 and take the
+//          two of the head's own (2^-22 of its largest); the sums of a group are f32 and take the
 //          token's scale there.
 //   softmax of head n over the lane's tokens 4g + r and 16 + 4g + r, in f32.
 //          The maximum and the exponent below are renewed, and O rescaled, only
@@ -316,7 +316,7 @@ __global__ __launch_bounds__(64 * TfKv8<HD>::W) void tf_flash_kv8_kernel(
     asm volatile("" ::: "memory");
 
     // the query of head n: dims 32 j + 8 g .. + 7 as two f16 parts of q 2^-e, the
-    // largest of the group's heads in [2^14, 2^15)
+    // head's largest in [2^14, 2^15) (an infinite one stays in its head)
     tf_h16x8 qa[NG][2];
     {
         const float* ql = reinterpret_cast<const float*>(lds + L::SLOT) + n * HD + 8 * g;
@@ -334,7 +334,8 @@ __global__ __launch_bounds__(64 * TfKv8<HD>::W) void tf_flash_kv8_kernel(
         for (int j = 0; j < NG; j++)
 #pragma unroll
             for (int i = 0; i < 8; i++) qmax = fmaxf(qmax, fabsf(qv[j][i]));
-        qmax = tf_wave_max(qmax);
+        qmax = fmaxf(qmax, __shfl_xor(qmax, 16));
+        qmax = fmaxf(qmax, __shfl_xor(qmax, 32));
         int fe = 141 - (int)(__float_as_uint(qmax) >> 23);
         fe = fe > 126 ? 126 : fe < -113 ? -113 : fe;
         const float f = __uint_as_float((uint32_t)(fe + 127) << 23);

@@ -254,3 +254,24 @@ def test_attention_whose_maximum_keeps_rising(gpu, h, kv, hd, seq, n_split):
     v8, vd = cache(rng, seq, kv * hd)
     got = attend(q, dev(k8), dev(kd), dev(v8), dev(vd), kv, seq - 1, n_split, scale)[0]
     check(got, q, ref.q8_values(k8, kd), ref.q8_values(v8, vd), kv, scale)
+
+
+@pytest.mark.parametrize("h,kv,hd", [(16, 2, 128), (14, 2, 64), (6, 2, 256)])
+@pytest.mark.parametrize("bad", [np.inf, -np.inf, np.nan, 3e38])
+def test_a_query_that_is_not_finite_stays_in_its_head(gpu, h, kv, hd, bad):
+    rng = np.random.default_rng(hd)
+    seq, scale = 500, 1 / np.sqrt(hd)
+    q = rng.standard_normal((h, hd)).astype(np.float32)
+    k8, kd = cache(rng, seq, kv * hd)
+    v8, vd = cache(rng, seq, kv * hd)
+    at = h // kv - 1
+    q[at, 7] = bad
+    rest = q.copy()
+    rest[at] = 0
+    want, tol = ref.attention(rest, ref.q8_values(k8, kd), ref.q8_values(v8, vd), kv, scale)
+    others = np.arange(h) != at
+    for n_split in (1, 8):
+        got = attend(q, dev(k8), dev(kd), dev(v8), dev(vd), kv, seq - 1, n_split, scale)[0]
+        assert (np.abs(got - want)[others] <= tol[others]).all()
+        if not np.isfinite(bad):
+            assert np.isnan(got[at]).all()
