@@ -141,10 +141,11 @@ __global__ __launch_bounds__(256) void tf_kv8_read_kernel(const int8_t* __restri
 //          The maximum and the exponent below are renewed, and O rescaled, only
 //          where a lane found a larger one.
 //   V^T P^T with the tokens in the order in which the lane has them: A = 8 tokens
-//          of dim n (ds_read_b64_tr_b8), as f16 (exact); B = p vd[t][g] 2^f, for
-//          each group of dims, in two f16 parts.  f takes the largest scale met
-//          so far to [2^14, 2^15), so the parts end at 2^-39 of the largest
-//          product.
+//          of dim n (ds_read_b64_tr_b8), as f16 (exact); B = p vd[t][g] f, for each
+//          group of dims, in two f16 parts.  f is a power of two of the head's that
+//          keeps every p vd f below 2^15 and the largest met so far (in the weights of
+//          the maximum so far) within 2^12 of that, so the parts end at 2^-28 of the
+//          largest product or below, whatever the scales of rows without weight.
 // 131072 tokens of 28/4 heads of 128 (151 MB): 36 us and 4.7 for the merge, 4.2 TB/s of
 // the 5.8 that a plain read reaches; the copies alone take 30, and conversions, splits
 // and exponentials keep the VALU busy for 17 beside them.  5001 tokens of
@@ -356,7 +357,8 @@ __global__ __launch_bounds__(64 * TfKv8<HD>::W) void tf_flash_kv8_kernel(
     if (wave + W < n_tiles) issue(wave + W, 1);
 
     float m = TF_NEG_BIG, l = 0.f;  // head n: the maximum, this lane's share of the sum
-    float vtop = 0.f, vf = 1.f;     // scales below vtop fit under the factor vf
+    // of head n: the largest weighted scale met, as of m; those below vtop fit under vf
+    float vmost = 0.f, vtop = 0.f, vf = 0x1p26f;
     tf_f32x4v o[DB];                // O^T of dims 16 b + 4 g + r, head n, times vf
 #pragma unroll
     for (int b = 0; b < DB; b++) o[b] = tf_f32x4v{0.f, 0.f, 0.f, 0.f};
@@ -418,13 +420,15 @@ __global__ __launch_bounds__(64 * TfKv8<HD>::W) void tf_flash_kv8_kernel(
                 sv[u][r] = t0 + 16 * u + 4 * g + r < t_end ? x : -INFINITY;
             }
         }
-        float top = 0.f, tm = sv[0][0];
+        float tt[2][4], top = 0.f, tm = sv[0][0];  // tt: a token's largest scale
 #pragma unroll
         for (int u = 0; u < 2; u++)
 #pragma unroll
             for (int r = 0; r < 4; r++) {
+                tt[u][r] = vsc[u][r][0];
 #pragma unroll
-                for (int i = 0; i < NG; i++) top = fmaxf(top, vsc[u][r][i]);
+                for (int i = 1; i < NG; i++) tt[u][r] = fmaxf(tt[u][r], vsc[u][r][i]);
+                top = fmaxf(top, tt[u][r]);
                 tm = fmaxf(tm, sv[u][r]);
             }
         if (__ballot(tm > m) | __ballot(top >= vtop)) {
@@ -434,15 +438,38 @@ __global__ __launch_bounds__(64 * TfKv8<HD>::W) void tf_flash_kv8_kernel(
             const float m_new = fmaxf(m, tm);
             const float alpha = __expf(m - m_new);
             float re = alpha;
-            if (top >= vtop) {  // wave-uniform; a larger maximum alone leaves the factor
-                // the power of two that takes scales up to `top` below 2^15
-                int fe = 141 - (int)(__float_as_uint(top) >> 23);
-                fe = fe > 126 ? 126 : fe < -126 ? -126 : fe;
-                const float f = __uint_as_float((uint32_t)(fe + 127) << 23);
-                // the first factor is whatever O = 0 takes
-                re *= vtop > 0.f ? f / vf : 1.f;
+            vmost *= alpha;
+            if (__ballot(top >= vtop) | __ballot(vmost < vtop * 0x1p-5f)) {
+                // Where the tile's scales are within 8 of each other and one of its tokens
+                // has a weight of e^-2 or more, the largest weighted one is within 2^6 of
+                // the largest; else it is formed.
+                float low = INFINITY;
+#pragma unroll
+                for (int u = 0; u < 2; u++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) low = fminf(low, tt[u][r]);
+                low = -tf_wave_max(-low);
+                if (__ballot(low * 8.f < top || tm < m_new - 2.f)) {
+                    float most = 0.f;
+#pragma unroll
+                    for (int u = 0; u < 2; u++)
+#pragma unroll
+                        for (int r = 0; r < 4; r++)
+                            most = fmaxf(most, tt[u][r] * __builtin_amdgcn_exp2f(
+                                                   (sv[u][r] - m_new) * 1.44269504088896340736f));
+                    most = fmaxf(most, __shfl_xor(most, 16));
+                    most = fmaxf(most, __shfl_xor(most, 32));
+                    top = fminf(top, most * 64.f);
+                }
+                vmost = fmaxf(vmost, top);
+                // the power of two that takes products up to vmost below 2^15
+                int fe = 141 - (int)(__float_as_uint(vmost) >> 23);
+                fe = fe > 126 ? 126 : fe < -113 ? -113 : fe;
+                // (by no more than 2^100 at once: the quotient is finite)
+                const float f = fminf(__uint_as_float((uint32_t)(fe + 127) << 23), vf * 0x1p100f);
+                re *= f / vf;
                 vf = f;
-                vtop = fe <= -113 ? INFINITY : __uint_as_float((uint32_t)(142 - fe) << 23);
+                vtop = __uint_as_float((269u << 23) - __float_as_uint(f));  // 2^15 / f
             }
             m = m_new;
             l *= alpha;

@@ -275,3 +275,38 @@ def test_a_query_that_is_not_finite_stays_in_its_head(gpu, h, kv, hd, bad):
         assert (np.abs(got - want)[others] <= tol[others]).all()
         if not np.isfinite(bad):
             assert np.isnan(got[at]).all()
+
+
+@pytest.mark.parametrize("h,kv,hd", [(16, 2, 128), (14, 2, 64), (6, 2, 256)])
+@pytest.mark.parametrize("big", [1e6, 1e15, 1e30])
+@pytest.mark.parametrize("case", ["unseen", "by_one_head", "seen_before_a_rise"])
+def test_attention_of_values_far_apart(gpu, h, kv, hd, big, case):
+    """Tokens, alone and by whole tiles of 32, whose values are larger than the others' by
+    more than f16 products hold: of no weight; of all the weight in one head and none in the
+    others; and of weight until later keys outweigh them."""
+    rng = np.random.default_rng(hd)
+    seq, n, scale = 900, kv * hd, 1 / np.sqrt(hd)
+    q = rng.standard_normal((h, hd)).astype(np.float32)
+    k = 0.1 * rng.standard_normal((seq, kv, hd))
+    v = rng.standard_normal((seq, n)).astype(np.float32)
+    at = [5, *range(288, 352), 899]
+    if case == "seen_before_a_rise":
+        at = [1]
+        k[600:] += 150 * (q.reshape(kv, -1, hd).mean(1) / (q.reshape(kv, -1, hd).mean(1)**2).sum(
+            -1, keepdims=True) / scale)
+    for r in at:
+        if case == "unseen":  # 150 below for all heads, by a channel that they share
+            q[:, 0] = 3
+            k[r] = 0
+            k[r, :, 0] = -50 / scale
+        elif case == "by_one_head":
+            q[:, 0] = 3
+            q[::h // kv, 0] = -3
+            k[r] = 0
+            k[r, :, 0] = -50 / scale
+    v[at] *= np.float32(big)
+    k8, kd = ref.q8_rows(k.reshape(seq, n).astype(np.float32))
+    v8, vd = ref.q8_rows(v)
+    for n_split in (1, 4):
+        got = attend(q, dev(k8), dev(kd), dev(v8), dev(vd), kv, seq - 1, n_split, scale)[0]
+        check(got, q, ref.q8_values(k8, kd), ref.q8_values(v8, vd), kv, scale)
