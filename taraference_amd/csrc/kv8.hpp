@@ -1,6 +1,14 @@
-// The 8-bit K/V cache's quantizer, shared by the kernels that write rows.
+// The 8-bit K/V cache's quantizer, shared by the kernels that write rows, and the
+// decode step's append.
 #pragma once
 #include "tf_common.hpp"
+
+// tf_rope_neox of q and k (the reference's f32 angle, which prompts have too, so that one
+// cache has one rotation) with k and v appended to the 8-bit cache, for one token.
+// head_dim 64, 128 or 256; 16-byte aligned.
+int tf_rope_append_kv8(float* q, const float* k, const float* v, int8_t* k8, float* kd, int8_t* v8,
+                       float* vd, int n_head, int n_kv, int head_dim, int pos, const int* pos_dev,
+                       float theta, tf_stream_t stream);
 
 // N values of a 32-value group with the largest magnitude amax: their int8, four a word,
 // and the group's scale; as tf_quantize_q8.

@@ -31,6 +31,7 @@
 #include "argmax_key.hpp"
 #include "decode_persistent.hpp"
 #include "gemv_b32.hpp"
+#include "kv8.hpp"
 #include "op_api.hpp"
 #include "prefill.hpp"
 #include "taraference_hip.h"
@@ -252,11 +253,9 @@ struct tf_model {
                 }
             }
             if (!kv8.empty())
-                tf::check(tf_qk_norm_rope_append_kv8(
-                              q, c.n_head * c.head_dim, k, c.n_kv * c.head_dim, v,
-                              c.n_kv * c.head_dim, nullptr, nullptr, 0.f, q, kv8[li].k8, kv8[li].kd,
-                              kv8[li].v8, kv8[li].vd, c.n_head, c.n_kv, c.head_dim, 1, pos, pos_dev,
-                              c.rope_theta, s),
+                tf::check(tf_rope_append_kv8(q, k, v, kv8[li].k8, kv8[li].kd, kv8[li].v8, kv8[li].vd,
+                                             c.n_head, c.n_kv, c.head_dim, pos, pos_dev,
+                                             c.rope_theta, s),
                           "rope + append kv8");
             else
                 tf::check(tf_rope_append(q, k, v, kc[li], vc[li], c.n_head, c.n_kv, c.head_dim, pos,

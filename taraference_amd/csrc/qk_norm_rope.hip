@@ -33,6 +33,7 @@ struct QkArgs {
     int pos0;
     const int* pos0_dev;
     double log2_theta;
+    float theta;
 };
 
 // Turns of pair i at position pos, less their whole part.
@@ -52,7 +53,8 @@ __device__ __forceinline__ float turns(long long pos, int i, int head_dim, doubl
 // Bound by its bytes: 4096 tokens of 28 + 8 heads of 128 into the 8-bit cache move 139
 // MB in 30.4 us (4.6 TB/s); 777 tokens of 16 + 2 heads of 128 to f32 rows 8.9 us, one
 // token of 14 + 2 heads of 64 4.0, which is a launch's chain of loads.
-template <int HD, Dest D, int TOK>
+// F32: the angle as tf_rope_neox and the prompts' kernels form it.
+template <int HD, Dest D, int TOK, bool F32 = false>
 __global__ __launch_bounds__(256) void tf_qk_norm_rope_vec_kernel(QkArgs a, int n_tok, int share) {
     constexpr int HALF = HD / 2, LPH = HD / 8, HEADS = 256 / LPH;
     __shared__ __align__(16) float cs[2][TOK][HALF];
@@ -95,7 +97,12 @@ __global__ __launch_bounds__(256) void tf_qk_norm_rope_vec_kernel(QkArgs a, int 
     for (int i = tid; i < TOK * HALF; i += 256) {
         const int tt = i / HALF, pair = i % HALF;
         float s, c;
-        sincospif(2.f * turns((long long)pos0 + tok0 + tt, pair, HD, a.log2_theta), &s, &c);
+        if constexpr (F32) {
+            const float freq = powf(a.theta, -2.f * (float)pair / (float)HD);
+            sincosf((float)(pos0 + tok0 + tt) * freq, &s, &c);
+        } else {
+            sincospif(2.f * turns((long long)pos0 + tok0 + tt, pair, HD, a.log2_theta), &s, &c);
+        }
         cs[0][tt][pair] = c;
         cs[1][tt][pair] = s;
     }
@@ -280,6 +287,32 @@ int launch(const QkArgs& a, int n_tok, float theta, tf_stream_t stream) {
 }
 
 }  // namespace
+
+int tf_rope_append_kv8(float* q, const float* k, const float* v, int8_t* k8, float* kd, int8_t* v8,
+                       float* vd, int n_head, int n_kv, int head_dim, int pos, const int* pos_dev,
+                       float theta, tf_stream_t stream) {
+    TF_CHECK_ARG(n_head > 0 && n_kv > 0 && n_head + 2LL * n_kv <= 65535 && head_dim > 0 &&
+                 (pos_dev || pos >= 0));
+    TF_CHECK_ARG((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v) & 15) == 0 &&
+                 (((uintptr_t)k8 | (uintptr_t)v8) & 3) == 0);
+    QkArgs a{};
+    a.q = q, a.k = k, a.v = v;  // one token: no strides
+    a.q_out = q, a.k8 = k8, a.kd = kd, a.v8 = v8, a.vd = vd;
+    a.n_head = n_head, a.n_kv = n_kv, a.head_dim = head_dim;
+    a.pos0 = pos, a.pos0_dev = pos_dev, a.theta = theta;
+    const int heads = n_head + 2 * n_kv, share = 2048 / head_dim;
+    auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3(1, (heads + share - 1) / share), dim3(256), 0,
+                           tf_stream(stream), a, 1, share);
+        return TF_LAUNCH_RESULT();
+    };
+    switch (head_dim) {
+    case 64: return go(tf_qk_norm_rope_vec_kernel<64, kKv8, 1, true>);
+    case 128: return go(tf_qk_norm_rope_vec_kernel<128, kKv8, 1, true>);
+    case 256: return go(tf_qk_norm_rope_vec_kernel<256, kKv8, 1, true>);
+    }
+    return (int)hipErrorInvalidValue;
+}
 
 extern "C" int tf_qk_norm_rope(const float* q, int q_stride, const float* k, int k_stride,
                                const float* q_norm, const float* k_norm, float eps, float* q_out,

@@ -168,3 +168,35 @@ def test_refusals(gpu):
     with pytest.raises(capi.HipError):
         gm.kv_cache(0, 1)
     gm.close()
+
+
+@pytest.mark.parametrize("pos", [0, 32000, 130000])
+def test_steps_and_prompts_turn_rows_alike(gpu, pos):
+    """A token's K row is turned by one angle whether a step or a prompt stores it, in 8 bits
+    or in f16.  Layer 0's input is the embedding's row, so a step's rows are the same numbers
+    in both caches: apart by half a step of each, and the rotation's roundings."""
+    cfg, layers, emb, make = build(0, 11, pos + 24)
+    f16, gm = make(), make()
+    gm.use_kv8()
+    f16.set_path(0)
+    toks = np.random.default_rng(pos).integers(0, cfg["n_vocab"], 24).tolist()
+    f16.generate(toks, 1, pos0=pos)
+    gm.generate(toks, 1, pos0=pos)
+    rows16 = [a[pos:].view(np.float16).astype(np.float64) for a in f16.kv_cache(0, pos + 24)]
+    k8, kd, v8, vd = (a[pos:] for a in gm.kv8_cache(0, pos + 24))
+    for q, d, want in ((k8, kd, rows16[0]), (v8, vd, rows16[1])):
+        step, got = np.repeat(d.astype(np.float64), 32, axis=1), ref.q8_values(q, d)
+        near = 2.0**-11 * np.abs(want) * (1 + 2.0**-10) + 2.0**-25
+        near = near + 2.0**-21 * np.abs(want).max(1, keepdims=True)
+        assert (np.abs(got - want) <= (0.5 + 2.0**-15) * step + near).all()
+    # the same tokens as a prompt (whose GEMMs take x unquantised, the steps' GEMVs its Q8):
+    # the f16 rows' Q8, exactly
+    f16.prefill(toks, pos)
+    gm.prefill(toks, pos)
+    rows16 = [a[pos:].view(np.float16).astype(np.float32) for a in f16.kv_cache(0, pos + 24)]
+    k8, kd, v8, vd = (a[pos:] for a in gm.kv8_cache(0, pos + 24))
+    for q, d, rows in ((k8, kd, rows16[0]), (v8, vd, rows16[1])):
+        want = ref.q8_rows(rows)
+        assert np.array_equal(q, want[0]) and np.array_equal(d, want[1])
+    f16.close()
+    gm.close()
