@@ -533,7 +533,8 @@ int tf_flash_decode_kv8_n_split(int n_kv, int head_dim, int max_seq);
  * logits (ties by rising index), top_k keeps the first k; top_p of these the
  * shortest run whose sum reaches p of theirs; min_p of these those with w >=
  * min_p.  out_idx = the first kept index in vocabulary order at which the
- * running sum of kept w exceeds u times their sum.
+ * running sum of kept w exceeds u times their sum (with a filter and u >= 2^-20
+ * the sums take each w to 2^-44 of the largest).
  * temperature, top_k, top_p, min_p: a value a row, or NULL (1, off, off, off);
  * top_k <= 0 or >= n_vocab, top_p >= 1 and min_p <= 0 (and NaN) are off,
  * top_p <= 0 keeps one token, min_p > 1 counts as 1; temperature <= 0 (or NaN)

@@ -30,11 +30,11 @@
 //   3. draw: a workgroup a row takes the cuts from the list, finds the segments in
 //      which the running sum passes u, and walks those.
 // Without top-k, top-p and min-p the second launch is left out.  A row whose cut lies
-// among more elements than the list holds (equal logits by the thousand), or whose logits
-// the bins cannot hold (an infinite one, T below 1e-37), is selected by radix passes over
-// the row itself in the third launch: the same cut, found by one workgroup (151936 equal
-// logits with top-p 312 us).  Bins of the row's own size keep others from there: logits
-// within 0.1 of each other, or T = 3, take the time of any row.
+// among more elements than the list holds (equal logits by the thousand), whose logits
+// the bins cannot hold (an infinite one, T below 1e-37), or whose u is below 2^-20, is
+// selected by radix passes over the row itself in the third launch: the same cut, found by
+// one workgroup (151936 equal logits with top-p 312 us).  Bins of the row's own size keep
+// others from there: logits within 0.1 of each other, or T = 3, take the time of any row.
 //
 // One row of 151936 with all filters: 9 + 8 + 4.5 us, without filters 5.6 + 4.5; bound by
 // chains of loads and barriers (19 workgroups, then one).  64 rows with top-p: 23.2 + 19.9
@@ -149,22 +149,23 @@ struct Settings {
     __device__ bool filtered() const { return use_k || use_p; }
     __device__ bool plain() const { return !use_k && !use_p && !(min_w > 0.0); }
 };
+// A row's value of a setting, or `off`: one value a workgroup, read by a scalar load, which
+// waits for no vector load, and branches on it are scalar too.
+template <class T>
+__device__ __forceinline__ T scalar_at(const T* p, int row, T off) {
+    typedef const __attribute__((address_space(4))) T Const;
+    return p ? ((Const*)(uintptr_t)p)[row] : off;
+}
 __device__ __forceinline__ Settings settings(const SampleArgs& a, int row) {
-    // one value a workgroup, read by scalar loads: they wait for no vector load, and
-    // branches on them are scalar too
-    auto at = [row](auto* p, auto off) {
-        typedef const __attribute__((address_space(4))) decltype(off) Const;
-        return p ? ((Const*)(uintptr_t)p)[row] : off;
-    };
     auto uni = [](float v) { return tf_readlane(v, 0); };
     Settings s;
-    s.temp = uni(at(a.temperature, 1.f));
+    s.temp = uni(scalar_at(a.temperature, row, 1.f));
     s.greedy = !(s.temp > 0.f);
-    s.k = __builtin_amdgcn_readfirstlane(at(a.top_k, 0));
+    s.k = __builtin_amdgcn_readfirstlane(scalar_at(a.top_k, row, 0));
     s.use_k = s.k > 0 && s.k < a.n;
-    s.p = uni(at(a.top_p, 1.f));
+    s.p = uni(scalar_at(a.top_p, row, 1.f));
     s.use_p = s.p < 1.f;
-    const float m = uni(at(a.min_p, 0.f));
+    const float m = uni(scalar_at(a.min_p, row, 0.f));
     s.min_w = m > 0.f ? fmin((double)m, 1.0) : 0.0;
     s.per_l = uni(kPerZ / s.temp);
     s.bad = !(s.temp >= 1e-37f);
@@ -873,6 +874,13 @@ __global__ __launch_bounds__(kRowThreads) void tf_sample_draw_kernel(SampleArgs 
     if (s.plain()) info.cut = 0, info.wide = 0;
     // the list's length and each chunk's place in it; too long for LDS, or a chunk's for
     // its room: the row itself
+    // A u below 2^-20 may fall among weights that the sums' unit of 2^-44 rounds away, or into
+    // a part whose weights are all below 2^-1000: such a row takes its sums, and its cut,
+    // from its logits.  Past it the rounding, 2^-26 for a whole row, is below 2^-6 of u.
+    float u = tf_readlane(scalar_at(a.u, row, 0.f), 0);
+    u = u > 0.f ? u : 0.f;  // NaN: 0
+    const bool small = u < 0x1p-20f;
+    if (small) info.cut = s.filtered() ? 2 : 0, info.wide = 0;
     int list_upto = 0, count = 0;
     if (info.cut == 1) {
         list_upto = wave_scan(mine_c.listed);
@@ -1007,7 +1015,8 @@ __global__ __launch_bounds__(kRowThreads) void tf_sample_draw_kernel(SampleArgs 
         }
         return ahead + upto;
     };
-    if (w.inf || info.cut == 2) {  // the segments' sums are not there: form them
+    const bool formed = w.inf || info.cut == 2 || small;
+    if (formed) {  // the segments' sums are not there: form them
         __syncthreads();
         for (int g = wave; g < segments; g += kRowWaves) {
             double v = 0.0;
@@ -1021,7 +1030,7 @@ __global__ __launch_bounds__(kRowThreads) void tf_sample_draw_kernel(SampleArgs 
     double seg_w = 0.0;
     if (tid < segments) {
         const u64 b = seg_sum[tid];
-        if (w.inf || info.cut == 2) {
+        if (formed) {
             seg_w = __builtin_bit_cast(double, b);
         } else if (s.plain()) {  // its chunk's largest -> the row's
             const float top = row_stats(a, row)[tid * kSegment / kBlock].top;
@@ -1032,9 +1041,7 @@ __global__ __launch_bounds__(kRowThreads) void tf_sample_draw_kernel(SampleArgs 
     }
     double total;
     const double upto = scan(0, seg_w, total);
-    double u = (double)a.u[row];
-    u = u > 0.0 ? u : 0.0;  // NaN: 0
-    const double target = u * total;
+    const double target = (double)u * total;
     // the first that passes the target (rounding may leave none: the last with a weight)
     auto choose = [&](int which, bool passes, int at, bool any, int last) {
         const u64 hits = __ballot(passes), has = __ballot(any);

@@ -246,3 +246,25 @@ def test_chunks_of_many_spreads(gpu):
             us = rng.random(8).astype(np.float32)
             a = {**a, "t": [t] * 8}
             assert np.array_equal(draw(gpu, x, us, **a), want(x, us, **a)), a
+
+
+@pytest.mark.parametrize("n,top", [(1500, 1200), (20000, 9000)])
+def test_small_u_with_filters(gpu, n, top):
+    """Kept weights far below the largest, of which a small u draws one: every token but one
+    has 4e-18 of its weight, the first of them 2e-15."""
+    x = np.zeros((1, n), np.float32)
+    x[0, top] = 40
+    x[0, 700] = 6
+    for u in (0.0, 1e-30, 2e-17, 1e-15, 3e-15, 1e-7, 9e-7, 1e-6, 0.5):
+        for a in ({}, {"m": [1e-18]}, {"k": [n - 100]}, {"k": [n - 100], "m": [4e-18]},
+                  {"k": [n - 100], "m": [1e-17]}, {"p": [0.5]}, {"k": [n - 1], "p": [0.99]}):
+            assert np.array_equal(draw(gpu, x, [u], **a), want(x, np.float32([u]), **a)), (u, a)
+
+
+def test_u_of_zero_among_weights_that_are_never_drawn(gpu):
+    """Weights below 2^-1000 (index 10: 2^-1040) are never drawn, in a part of the row whose
+    largest (index 2100: 2^-577) is far below the row's."""
+    x = np.full((1, 16384), -np.inf, np.float32)
+    x[0, 10], x[0, 2100], x[0, 9000] = -1040 * np.log(2), -577 * np.log(2), 0
+    for a in ({}, {"m": [1e-45]}, {"k": [3]}):
+        assert draw(gpu, x, [0.0], **a)[0] == (9000 if "m" in a else 2100), a
