@@ -464,7 +464,8 @@ int tf_argmax_key_finalize(unsigned long long *amax_key, int *out_idx,
  * No counterpart in the reference.  An 8-bit cache row is the Q8 of
  * tf_quantize_q8: int8 k8[seq][n] and f32 kd[seq][n/32] (v8, vd alike), n =
  * n_kv*head_dim, d = amax * fl(1/127), q = rint_even(x / d), value = q * d:
- * 36 bytes per 32 values where f16 takes 64.  Values are finite. */
+ * 36 bytes per 32 values where f16 takes 64.  Values are finite.  Where a device
+ * position is negative, rows at positions below 0 are not written. */
 
 #define TF_KV_F32 0 /* element types of the rows written and read back */
 #define TF_KV_F16 1

@@ -37,7 +37,9 @@ __global__ __launch_bounds__(256) void tf_kv8_write_kernel(TfKv8Rows a) {
     const size_t e = ((size_t)blockIdx.x * 256 + threadIdx.x) * PER;
     if (e >= a.count) return;  // whole groups: count % 32 == 0
     const bool is_v = blockIdx.y == 1;
-    const size_t at = (size_t)(a.pos0_dev ? a.pos0_dev[0] : a.pos0) * a.n + e;
+    const long long to = (long long)(a.pos0_dev ? a.pos0_dev[0] : a.pos0) * a.n + (long long)e;
+    if (to < 0) return;  // a row before the cache
+    const size_t at = (size_t)to;
     size_t from = e;  // tight rows
     if (a.stride != a.n) {
         const size_t t = e >> 32 == 0 ? (uint32_t)e / (uint32_t)a.n : e / a.n;

@@ -153,7 +153,9 @@ __global__ __launch_bounds__(256) void tf_qk_norm_rope_vec_kernel(QkArgs a, int 
             *reinterpret_cast<float4*>(out + 4 * m + HALF) = make_float4(v[4], v[5], v[6], v[7]);
             continue;
         }
-        const size_t at = ((size_t)((long long)pos0 + t_now) * a.n_kv + h_now) * HD + 4 * m;
+        const long long pos = (long long)pos0 + t_now;
+        if (pos < 0) continue;  // no place in the cache
+        const size_t at = ((size_t)pos * a.n_kv + h_now) * HD + 4 * m;
 #pragma unroll
         for (int i = 0; i < 2; i++) {
             const float y[4] = {v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]};
@@ -227,6 +229,7 @@ __global__ __launch_bounds__(256) void tf_qk_norm_rope_kernel(QkArgs a) {
         for (int i = lane; i < hd; i += 64) out[i] = y[i];
         return;
     }
+    if (pos < 0) return;  // no place in the cache
     const size_t at = ((size_t)pos * a.n_kv + h) * hd;
     if (D == kF16) {
         uint16_t* c = (kind == 1 ? a.kc : a.vc) + at;

@@ -310,3 +310,39 @@ def test_attention_of_values_far_apart(gpu, h, kv, hd, big, case):
     for n_split in (1, 4):
         got = attend(q, dev(k8), dev(kd), dev(v8), dev(vd), kv, seq - 1, n_split, scale)[0]
         check(got, q, ref.q8_values(k8, kd), ref.q8_values(v8, vd), kv, scale)
+
+
+@pytest.mark.parametrize("dest", ["f16", "kv8", "write", "write_off_alignment"])
+def test_rows_at_negative_positions_are_left(gpu, dest):
+    """*pos0_dev = -2: the first two of the rows have no place, the others go to 0, 1, .."""
+    h, kv, hd, t, spare = 4, 2, 64, 5, 4
+    n, w = kv * hd, (h + 2 * kv) * hd
+    x = np.random.default_rng(8).standard_normal((t, w)).astype(np.float32)
+    d, pos, qo = dev(x), dev(np.array([-2], np.int32)), empty(t * h * hd)
+    off = 1 if dest == "write_off_alignment" else 0
+    k8, v8 = (dev(np.full((spare + t) * n + off, 77, np.int8)) for _ in range(2))
+    kd, vd = (dev(np.full((spare + t) * n // 32, -3, np.float32)) for _ in range(2))
+    kc, vc = (dev(np.full((spare + t) * n, 0x1234, np.uint16)) for _ in range(2))
+    c8 = (P(k8) + spare * n + off, P(kd) + spare * n // 8, P(v8) + spare * n + off,
+          P(vd) + spare * n // 8)
+    pk, pv = P(d) + 4 * h * hd, P(d) + 4 * (h + kv) * hd
+    rows = (P(d), w, pk, w, pv, w, None, None, 1e-6, P(qo))
+    tail = (h, kv, hd, t, 0, P(pos), 1e4, S())
+    if dest == "f16":
+        call("tf_qk_norm_rope_append", *rows, P(kc) + 2 * spare * n, P(vc) + 2 * spare * n, *tail)
+    elif dest == "kv8":
+        call("tf_qk_norm_rope_append_kv8", *rows, *c8, *tail)
+    else:
+        call("tf_kv8_write", pk, pv, gpu.KV_F32, w, *c8, n, 0, P(pos), t, S())
+    v = np.ascontiguousarray(x[2:, (h + kv) * hd:])
+    if dest == "f16":
+        for c in (kc, vc):
+            assert (host(c)[:spare * n] == 0x1234).all() and (host(c)[(spare + t - 2) * n:] == 0x1234).all()
+        assert np.array_equal(host(vc)[spare * n:(spare + t - 2) * n], oracle.f32_to_f16(v.ravel()))
+        return
+    q8, d8 = ref.q8_rows(v)
+    for c, s, want, mark in ((k8, 1, None, 77), (v8, 1, q8, 77), (kd, 32, None, -3), (vd, 32, d8, -3)):
+        a, b = spare * n // s + (off if s == 1 else 0), (spare + t - 2) * n // s + (off if s == 1 else 0)
+        assert (host(c)[:a] == mark).all() and (host(c)[b:] == mark).all()
+        if want is not None:
+            assert np.array_equal(host(c)[a:b], want.ravel())
