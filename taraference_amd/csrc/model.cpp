@@ -757,9 +757,10 @@ struct tf_model {
     // the token drawn from its logits by u[i].
     void run(hipStream_t s, const int* forced, int n_forced, int pos0, int n_gen, int* tokens,
              bool use_graph, const tf_sampling* how = nullptr, const float* u = nullptr) {
-        const int total = n_forced + (n_gen > 0 ? n_gen : 1) - 1;
-        if (n_forced < 1 || pos0 < 0 || pos0 + total > cfg.max_seq)
+        const long long steps = (long long)n_forced + (n_gen > 0 ? n_gen : 1) - 1;
+        if (n_forced < 1 || pos0 < 0 || pos0 + steps > cfg.max_seq)
             throw tf::HipError(1, "decode range outside the KV cache");
+        const int total = (int)steps;
         if (how) set_sampling(s, *how, u, n_gen);
         std::vector<int> h(4);
         h[0] = pos0;
@@ -831,7 +832,7 @@ struct tf_model {
     // launches: each GEMM's K slices are added by the kernel that reads them.
     void prefill(hipStream_t s, const int* tokens, int n, int pos0) {
         const tf_model_config& c = cfg;
-        if (n < 1 || pos0 < 0 || pos0 + n > c.max_seq)
+        if (n < 1 || pos0 < 0 || (long long)pos0 + n > c.max_seq)
             throw tf::HipError((int)hipErrorInvalidValue, "prefill range outside the KV cache");
         if (!kquant_ok())
             throw tf::HipError((int)hipErrorNotSupported, "prefill needs Q4_K/Q6_K weights");

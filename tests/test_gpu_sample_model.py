@@ -72,3 +72,21 @@ def test_refusals(gpu):
     import ctypes as C
     assert gm.lib.tf_model_sample(gm.h, None, 0.5, C.byref(C.c_int()), None) == 1
     gm.close()
+
+
+def test_ranges_past_32_bits(gpu):
+    """Positions and counts whose sum passes 2^31 are outside of the cache too."""
+    import ctypes as C
+    cfg = TINY[0]
+    gm, _ = build(cfg, 3, 32)
+    lib, h, last = gm.lib, gm.h, 2**31 - 1
+    from taraference_amd.model import TfSampling
+    how, out, u = TfSampling(1.0, 0, 1.0, 0.0), (C.c_int * 4)(), (C.c_float * 4)()
+    one = (C.c_int * 1)(5)
+    for pos0, n_gen in ((last, 1), (last, 2), (1, last), (last, last), (32, 1), (0, 33)):
+        assert lib.tf_model_generate_sampled(h, one, 1, pos0, n_gen, C.byref(how), u, out, 0, None) == 1
+        assert lib.tf_model_generate(h, one, 1, pos0, n_gen, out, 0, None) == 1
+    for pos0 in (last, 32):
+        with pytest.raises(capi.HipError):
+            gm.prefill([1, 2], pos0)
+    gm.close()
