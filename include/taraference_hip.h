@@ -643,13 +643,20 @@ int tf_model_generate_sampled(tf_model *m, const int *forced, int n_forced,
                               tf_stream_t stream);
 /* No counterpart in the reference: hold the K/V cache in 8 bits (see
  * tf_kv8_write) from here on, n_layer * max_seq * n_kv * head_dim * 2.25 bytes
- * in place of 4.  Rows written before are lost.  Steps take path 0 with their
- * rows stored in 8 bits, turned by tf_rope_neox's angle as prompts' are, and
- * tf_flash_decode_kv8 in it; prompts attend over the rows read back in f16, and
- * over their own as f16 has them, from which they are stored.  head_dim 64, 128 or 256, n_head / n_kv <= 16 (else
- * hipErrorNotSupported).  There is no way back; tf_model_set_path(1 .. 4) then
- * returns hipErrorNotSupported and tf_model_k_cache / v_cache NULL. */
+ * in place of 4; until this returns there is room for both.  Rows written before
+ * are lost.  Steps take path 0 with their rows stored in 8 bits, turned by
+ * tf_rope_neox's angle as prompts' are, and tf_flash_decode_kv8 in it; prompts
+ * attend over the rows read back in f16 (room for one layer's, taken on the first
+ * prompt), and over their own as f16 has them, from which they are stored.
+ * head_dim 64, 128 or 256, n_head / n_kv <= 16 (else hipErrorNotSupported).
+ * There is no way back; tf_model_set_path(1 .. 4) then returns
+ * hipErrorNotSupported and tf_model_k_cache / v_cache NULL. */
 int tf_model_use_kv8(tf_model *m);
+/* tf_model_create with that cache from the start: the f16 one is never
+ * allocated. */
+int tf_model_create_kv8(const tf_model_config *cfg, const tf_layer *layers,
+                        const tf_mat *token_embd, const tf_mat *output,
+                        const float *output_norm, tf_model **out);
 /* The 8-bit cache of layer li: part 0 = int8 k, 1 = f32 k scales, 2 = int8 v, 3 =
  * f32 v scales; NULL without one. */
 const void *tf_model_kv8_cache(const tf_model *m, int li, int part);

@@ -158,7 +158,7 @@ BOUND_ELSEWHERE = {"tf_model_create", "tf_model_destroy", "tf_model_forward",
                    "tf_model_stage_vector", "tf_model_q8_record",
                    "tf_model_k_cache", "tf_model_v_cache", "tf_exported_symbol",
                    "tf_sample_ws_bytes", "tf_model_sample", "tf_model_generate_sampled",
-                   "tf_model_use_kv8", "tf_model_kv8_cache",
+                   "tf_model_use_kv8", "tf_model_create_kv8", "tf_model_kv8_cache",
                    # taraference_amd/gguf.py
                    "tf_gguf_open", "tf_gguf_close", "tf_gguf_version", "tf_gguf_data_offset",
                    "tf_gguf_file_size", "tf_gguf_n_tensors", "tf_gguf_tensor_at",

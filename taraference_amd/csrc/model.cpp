@@ -114,9 +114,9 @@ struct tf_model {
     float* q8_d = nullptr;
     size_t partial_stride = 0;
     std::vector<uint16_t*> kc, vc;
-    // the 8-bit cache (tf_model_use_kv8): then kc and vc are empty, and k16 / v16 hold one
-    // layer's rows in f16 while a prompt attends over them (the earlier ones read back,
-    // its own as they are)
+    // the 8-bit cache (tf_model_create_kv8, tf_model_use_kv8): then kc and vc are empty, and
+    // k16 / v16, allocated on the first prompt, hold one layer's rows in f16 while it attends
+    // over them (the earlier ones read back, its own as they are)
     struct Kv8 {
         int8_t *k8, *v8;
         float *kd, *vd;
@@ -188,6 +188,29 @@ struct tf_model {
     void release(void* p) {
         allocs.erase(std::find(allocs.begin(), allocs.end(), p));
         (void)hipFree(p);
+    }
+
+    static bool kv8_takes(const tf_model_config& c) {
+        return (c.head_dim == 64 || c.head_dim == 128 || c.head_dim == 256) && c.n_head / c.n_kv <= 16;
+    }
+    // The 8-bit cache's rows and the partials of its attention; `mine` lists what is allocated.
+    void kv8_room(std::vector<Kv8>& made, float*& partial, std::vector<void*>& mine) {
+        const size_t n = (size_t)cfg.max_seq * cfg.n_kv * cfg.head_dim;
+        made.resize(cfg.n_layer);
+        mine.reserve(4 * made.size() + 1);
+        allocs.reserve(allocs.size() + mine.capacity());
+        auto room = [&](auto*& p, size_t count) {
+            p = alloc<std::remove_reference_t<decltype(*p)>>(count);
+            mine.push_back(p);
+        };
+        for (auto& l : made) {
+            room(l.k8, n);
+            room(l.v8, n);
+            room(l.kd, n / 32);
+            room(l.vd, n / 32);
+        }
+        kv8_split = tf_flash_decode_kv8_n_split(cfg.n_kv, cfg.head_dim, cfg.max_seq);
+        room(partial, (size_t)cfg.n_head * kv8_split * (2 + cfg.head_dim));
     }
 
     ~tf_model() {
@@ -849,6 +872,10 @@ struct tf_model {
             pf_ws = alloc<float>(pf_ws_floats);
             pf_x = alloc<float>((size_t)CH * E);
         }
+        if (!kv8.empty() && !v16) {
+            if (!k16) k16 = alloc<uint16_t>((size_t)c.max_seq * kvd);
+            v16 = alloc<uint16_t>((size_t)c.max_seq * kvd);
+        }
         const tf_stream_t ts = reinterpret_cast<tf_stream_t>(s);
         auto blk = [](const GpuMat& w) { return w.wtype == tf::WType::Q6K ? 210 : 144; };
         int last = 0;
@@ -950,14 +977,14 @@ struct tf_model {
     }
 };
 
-extern "C" int tf_model_create(const tf_model_config* cfg, const tf_layer* layers,
-                               const tf_mat* token_embd, const tf_mat* output,
-                               const float* output_norm, tf_model** out) {
+static int create(const tf_model_config* cfg, const tf_layer* layers, const tf_mat* token_embd,
+                  const tf_mat* output, const float* output_norm, bool kv8, tf_model** out) {
     if (!cfg || !layers || !token_embd || !output || !output_norm || !out) return (int)hipErrorInvalidValue;
     const tf_model_config& c = *cfg;
     if (c.n_layer <= 0 || c.n_embd % 32 || c.n_ff % 32 || c.n_head <= 0 || c.n_kv <= 0 ||
         c.n_head % c.n_kv || c.n_head * c.head_dim != c.n_embd || c.max_seq <= 0 || c.n_vocab <= 0)
         return (int)hipErrorInvalidValue;
+    if (kv8 && !tf_model::kv8_takes(c)) return (int)hipErrorNotSupported;
     try {
         std::unique_ptr<tf_model> m(new tf_model());
         m->cfg = c;
@@ -1000,11 +1027,16 @@ extern "C" int tf_model_create(const tf_model_config* cfg, const tf_layer* layer
         m->q8_d = m->alloc<float>(std::max(c.n_ff, c.n_embd) / 32);
         m->partial_stride = widest;
         m->gemv_partial = m->alloc<float>(8 * widest);
-        m->flash_partial = m->alloc<float>((size_t)c.n_head * n_split * (2 + c.head_dim));
-        const size_t kv_elems = (size_t)c.max_seq * c.n_kv * c.head_dim;
-        for (int i = 0; i < c.n_layer; i++) {
-            m->kc.push_back(m->alloc<uint16_t>(kv_elems));
-            m->vc.push_back(m->alloc<uint16_t>(kv_elems));
+        if (kv8) {
+            std::vector<void*> all;  // the model's own by now
+            m->kv8_room(m->kv8, m->flash_partial, all);
+        } else {
+            m->flash_partial = m->alloc<float>((size_t)c.n_head * n_split * (2 + c.head_dim));
+            const size_t kv_elems = (size_t)c.max_seq * c.n_kv * c.head_dim;
+            for (int i = 0; i < c.n_layer; i++) {
+                m->kc.push_back(m->alloc<uint16_t>(kv_elems));
+                m->vc.push_back(m->alloc<uint16_t>(kv_elems));
+            }
         }
         m->d_pos = m->alloc<int>(1);
         m->d_step = m->alloc<int>(1);
@@ -1020,7 +1052,7 @@ extern "C" int tf_model_create(const tf_model_config* cfg, const tf_layer* layer
         m->d_log = m->alloc<int>(c.max_seq);
         // the persistent step where the kernel serves this model, else the
         // fused multi-launch step
-        m->path = m->persistent_ok() ? 4 : (m->kquant_ok() ? 3 : 0);
+        m->path = kv8 ? 0 : m->persistent_ok() ? 4 : (m->kquant_ok() ? 3 : 0);
         *out = m.release();
         return 0;
     } catch (const tf::HipError& e) {
@@ -1028,6 +1060,18 @@ extern "C" int tf_model_create(const tf_model_config* cfg, const tf_layer* layer
     } catch (const std::bad_alloc&) {
         return (int)hipErrorOutOfMemory;
     }
+}
+
+extern "C" int tf_model_create(const tf_model_config* cfg, const tf_layer* layers,
+                               const tf_mat* token_embd, const tf_mat* output,
+                               const float* output_norm, tf_model** out) {
+    return create(cfg, layers, token_embd, output, output_norm, false, out);
+}
+
+extern "C" int tf_model_create_kv8(const tf_model_config* cfg, const tf_layer* layers,
+                                   const tf_mat* token_embd, const tf_mat* output,
+                                   const float* output_norm, tf_model** out) {
+    return create(cfg, layers, token_embd, output, output_norm, true, out);
 }
 
 extern "C" void tf_model_destroy(tf_model* m) { delete m; }
@@ -1124,35 +1168,16 @@ extern "C" int tf_model_generate_sampled(tf_model* m, const int* forced, int n_f
 extern "C" int tf_model_use_kv8(tf_model* m) {
     if (!m) return (int)hipErrorInvalidValue;
     if (!m->kv8.empty()) return 0;
-    const tf_model_config& c = m->cfg;
-    const int hd = c.head_dim;
-    if ((hd != 64 && hd != 128 && hd != 256) || c.n_head / c.n_kv > 16)
-        return (int)hipErrorNotSupported;
+    if (!tf_model::kv8_takes(m->cfg)) return (int)hipErrorNotSupported;
     std::vector<void*> mine;  // given back if anything fails: all that may comes first
     try {
-        const size_t n = (size_t)c.max_seq * c.n_kv * hd;
-        std::vector<tf_model::Kv8> made(c.n_layer);
-        mine.reserve(4 * made.size() + 1);
-        auto room = [&](auto*& p, size_t count) {
-            p = m->alloc<std::remove_reference_t<decltype(*p)>>(count);
-            mine.push_back(p);
-        };
-        for (auto& l : made) {
-            room(l.k8, n);
-            room(l.v8, n);
-            room(l.kd, n / 32);
-            room(l.vd, n / 32);
-        }
-        const int split = tf_flash_decode_kv8_n_split(c.n_kv, hd, c.max_seq);
+        std::vector<tf_model::Kv8> made;
         float* partial;
-        room(partial, (size_t)c.n_head * split * (2 + hd));
+        m->kv8_room(made, partial, mine);
         tf::check((int)hipDeviceSynchronize(), "sync");
-        m->kv8_split = split;
+        m->release(m->flash_partial);
         m->flash_partial = partial;
-        // one layer's f16 rows stay as the prompts' scratch
-        m->k16 = m->kc[0];
-        m->v16 = m->vc[0];
-        for (size_t i = 1; i < m->kc.size(); i++) {
+        for (size_t i = 0; i < m->kc.size(); i++) {
             m->release(m->kc[i]);
             m->release(m->vc[i]);
         }

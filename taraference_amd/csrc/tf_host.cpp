@@ -171,6 +171,7 @@ static const char* const k_symbols[] = {
     "tf_model_sample",
     "tf_model_generate_sampled",
     "tf_model_use_kv8",
+    "tf_model_create_kv8",
     "tf_model_kv8_cache",
     "tf_model_set_path",
     "tf_model_get_path",

@@ -48,6 +48,8 @@ def _bind(lib):
                                     C.POINTER(TfMat), C.POINTER(TfMat), C.c_void_p,
                                     C.POINTER(C.c_void_p)]
     lib.tf_model_create.restype = C.c_int
+    lib.tf_model_create_kv8.argtypes = lib.tf_model_create.argtypes
+    lib.tf_model_create_kv8.restype = C.c_int
     lib.tf_model_destroy.argtypes = [C.c_void_p]
     lib.tf_model_destroy.restype = None
     lib.tf_model_forward.argtypes = [C.c_void_p, C.c_int, C.c_int, C.POINTER(C.c_int),
@@ -98,11 +100,12 @@ class DecodeModel:
     when down_q6k), or (bytes, col_bytes, ggml type).  Biases may be None.
     embedding: the token table (a matrix, Q6_K unless typed); output: a
     separate lm_head (None: tied to the embedding); output_norm: the final
-    RMSNorm weight (None: ones).
+    RMSNorm weight (None: ones).  kv8: the K/V cache in 8 bits from the start
+    (see use_kv8), where the f16 one need not fit.
     """
 
     @classmethod
-    def from_gguf(cls, path, max_seq: int) -> "DecodeModel":
+    def from_gguf(cls, path, max_seq: int, kv8: bool = False) -> "DecodeModel":
         """cuda/load.rs:166-420 for a dense Qwen2/Llama Q4_K_M file: the
         config from the metadata (config.rs:107-175), blk.{i}.* tensors by
         the reference's names, a tied lm_head when output.weight is absent."""
@@ -169,11 +172,12 @@ class DecodeModel:
             emb = mat("token_embd.weight", c["n_embd"])
             out = mat("output.weight", c["n_embd"]) if f.tensor("output.weight") else None
             return cls(cfg, layers(), emb, output=out,
-                       output_norm=vec("output_norm.weight", c["n_embd"]))
+                       output_norm=vec("output_norm.weight", c["n_embd"]), kv8=kv8)
         finally:
             f.close()
 
-    def __init__(self, cfg: dict, layers, embedding, output=None, output_norm=None):
+    def __init__(self, cfg: dict, layers, embedding, output=None, output_norm=None,
+                 kv8: bool = False):
         self.lib = capi.load()
         _bind(self.lib)
         self.cfg = dict(cfg)
@@ -203,13 +207,14 @@ class DecodeModel:
                            c["head_dim"], c["n_vocab"], c["max_seq"], c["rope_theta"],
                            c["rms_eps"])
         h = C.c_void_p()
-        rc = self.lib.tf_model_create(C.byref(cc), carr, C.byref(self.embd), C.byref(self.out),
-                                      self.output_norm, C.byref(h))
+        create = self.lib.tf_model_create_kv8 if kv8 else self.lib.tf_model_create
+        rc = create(C.byref(cc), carr, C.byref(self.embd), C.byref(self.out), self.output_norm,
+                    C.byref(h))
         if rc != 0:
-            raise capi.HipError(f"tf_model_create returned {rc}")
+            raise capi.HipError(f"{create.__name__} returned {rc}")
         self.h = h
         self._layers = carr
-        self.kv8 = False
+        self.kv8 = kv8
         # the batched prefill takes K-quant matrices of widths that are multiples of 256
         mats = [self.embd, self.out] + [getattr(t, n) for t in carr for n in
                                         ("wq", "wk", "wv", "wo", "gate", "up", "down")]
@@ -433,7 +438,8 @@ class DecodeModel:
 
     def use_kv8(self) -> None:
         """Hold the K/V cache in 8 bits from here on (rows written before are
-        lost, steps take path 0): 0.5625 of the f16 cache's bytes."""
+        lost, steps take path 0): 0.5625 of the f16 cache's bytes, beside it
+        until this returns (DecodeModel(.., kv8=True) never allocates that)."""
         rc = self.lib.tf_model_use_kv8(self.h)
         if rc != 0:
             raise capi.HipError(f"tf_model_use_kv8 returned {rc}")

@@ -200,3 +200,44 @@ def test_steps_and_prompts_turn_rows_alike(gpu, pos):
         assert np.array_equal(q, want[0]) and np.array_equal(d, want[1])
     f16.close()
     gm.close()
+
+
+def test_the_8_bit_cache_takes_the_place_of_the_f16_one(gpu):
+    """A model made with it never holds the f16 cache, one that is switched gives it back;
+    both go on alike."""
+    from taraference_amd.model import DecodeModel
+    rows = 400_000
+    cfg, layers, emb, _ = build(0, 9, rows)
+
+    def make(**how):
+        return DecodeModel(dict(cfg, max_seq=rows), layers, emb, **how)
+
+    n = cfg["n_layer"] * rows * cfg["n_kv"] * cfg["head_dim"]
+    other = 64 << 20  # weights and workspaces
+
+    def used():
+        torch.cuda.synchronize()
+        return torch.cuda.mem_get_info()[1] - torch.cuda.mem_get_info()[0]
+
+    warm = build(0, 9, 64)[3]()
+    warm.prefill([1, 2, 3], 0)
+    warm.generate([4], 2, pos0=3)
+    warm.close()
+    base = used()
+    early = make(kv8=True)
+    assert early.path() == 0 and early.kv8
+    assert 2.25 * n <= used() - base < 2.25 * n + other
+    early.generate([3, 4, 5], 3)
+    assert used() - base < 2.25 * n + other
+    want, tok = early.logits(), early.generate([3, 4, 5], 3)
+    early.close()
+    base = used()
+    late = make()
+    late.forward(7, 0)
+    assert used() - base >= 4 * n
+    late.use_kv8()
+    assert used() - base < 2.25 * n + other
+    assert np.array_equal(late.generate([3, 4, 5], 3), tok) and np.array_equal(late.logits(), want)
+    late.prefill(list(range(20)), 0)
+    assert used() - base < 2.25 * n + 4 * n / cfg["n_layer"] + 2 * other  # and a layer in f16
+    late.close()

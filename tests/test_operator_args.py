@@ -141,3 +141,18 @@ def test_oracles_agree_with_themselves():
     assert np.allclose(y, 1.0)
     q, d = ref.q8_rows(np.arange(-16, 16, dtype=np.float32)[None])
     assert q[0, 0] == -127 and d.shape == (1, 1)
+
+
+@pytest.mark.parametrize("shape", [dict(n_embd=512, n_head=16, n_kv=16, head_dim=32),
+                                   dict(n_embd=2176, n_head=34, n_kv=2, head_dim=64)])
+def test_models_without_an_8_bit_cache(lib, shape):
+    """Heads that its attention does not take: refused before anything is allocated."""
+    from taraference_amd import model as M
+    M._bind(lib)
+    cfg = M.TfModelConfig(n_layer=1, n_ff=512, n_vocab=100, max_seq=8, rope_theta=1e4, rms_eps=1e-6,
+                          **shape)
+    out, mat = C.c_void_p(), M.TfMat()
+    args = (C.byref(cfg), (M.TfLayer * 1)(), C.byref(mat), C.byref(mat), A, C.byref(out))
+    assert lib.tf_model_create_kv8(*args) == 801  # hipErrorNotSupported
+    assert lib.tf_model_create_kv8(None, *args[1:]) == INVALID
+    assert not out.value and lib.tf_model_use_kv8(None) == INVALID
