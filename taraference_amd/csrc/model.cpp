@@ -92,7 +92,10 @@ __global__ void tf_decode_take_kernel(const int* drawn, const int* step, const i
 template <class T>
 T* dev_alloc(size_t n) {
     void* p = nullptr;
-    if (hipMalloc(&p, n * sizeof(T) + 256) != hipSuccess) throw std::bad_alloc();
+    if (hipMalloc(&p, n * sizeof(T) + 256) != hipSuccess) {
+        (void)hipGetLastError();  // reported by the exception, not by the next launch too
+        throw std::bad_alloc();
+    }
     return static_cast<T*>(p);
 }
 

@@ -241,3 +241,16 @@ def test_the_8_bit_cache_takes_the_place_of_the_f16_one(gpu):
     late.prefill(list(range(20)), 0)
     assert used() - base < 2.25 * n + 4 * n / cfg["n_layer"] + 2 * other  # and a layer in f16
     late.close()
+
+
+@pytest.mark.parametrize("kv8", [False, True])
+def test_a_cache_that_does_not_fit(gpu, kv8):
+    """Refused with hipErrorOutOfMemory, which the next launch does not report again."""
+    from taraference_amd.model import DecodeModel
+    cfg, layers, emb, make = build(1, 2, 16)
+    gm = make()
+    want = gm.generate([1, 2], 3, use_graph=False)
+    with pytest.raises(capi.HipError, match="returned 2$"):
+        DecodeModel(dict(cfg, max_seq=2**31 - 1), layers, emb, kv8=kv8)
+    assert np.array_equal(gm.generate([1, 2], 3, use_graph=False), want)
+    gm.close()
