@@ -1095,6 +1095,8 @@ extern "C" int tf_model_forward(tf_model* m, int token, int pos, int* next_token
         return 0;
     } catch (const tf::HipError& e) {
         return e.code;
+    } catch (const std::bad_alloc&) {
+        return (int)hipErrorOutOfMemory;
     }
 }
 
@@ -1109,6 +1111,8 @@ extern "C" int tf_model_generate(tf_model* m, const int* forced, int n_forced, i
         return 0;
     } catch (const tf::HipError& e) {
         return e.code;
+    } catch (const std::bad_alloc&) {
+        return (int)hipErrorOutOfMemory;
     }
 }
 
