@@ -1080,28 +1080,34 @@ long long row_bytes_of(int chunks) {
     return 128 + sizeof(ChunkStat) * kMaxChunks + 8LL * (kMaxSegments + (long long)chunks * kChunkWords);
 }
 
+int chunks_of(int n_vocab) { return (n_vocab + kBlock - 1) / kBlock; }
+
+// Sizes whose grids have fewer than 2^32 threads.
+bool sizes_ok(int n_rows, int n_vocab) {
+    return n_rows > 0 && n_vocab > 0 && n_vocab < kMaxVocab &&
+           (long long)n_rows * chunks_of(n_vocab) <= (long long)(UINT32_MAX / kRowThreads);
+}
+
 }  // namespace
 
 extern "C" long long tf_sample_ws_bytes(int n_rows, int n_vocab) {
-    if (n_rows <= 0 || n_vocab <= 0 || n_vocab >= kMaxVocab) return -1;
-    return n_rows * row_bytes_of((n_vocab + kBlock - 1) / kBlock);
+    return sizes_ok(n_rows, n_vocab) ? n_rows * row_bytes_of(chunks_of(n_vocab)) : -1;
 }
 
 extern "C" int tf_sample(const float* logits, int n_rows, int n_vocab, int row_stride,
                          const float* temperature, const int* top_k, const float* top_p,
                          const float* min_p, const float* u, int* out_idx, void* ws,
                          long long ws_bytes, tf_stream_t stream) {
-    TF_CHECK_ARG(logits && u && out_idx && ws && n_rows > 0 && n_vocab > 0);
-    TF_CHECK_ARG(n_vocab < kMaxVocab && row_stride >= n_vocab && ((uintptr_t)ws & 15) == 0);
+    TF_CHECK_ARG(logits && u && out_idx && ws && sizes_ok(n_rows, n_vocab));
+    TF_CHECK_ARG(row_stride >= n_vocab && ((uintptr_t)ws & 15) == 0);
     TF_CHECK_ARG(ws_bytes >= tf_sample_ws_bytes(n_rows, n_vocab));
     SampleArgs a{};
     a.logits = logits, a.stride = row_stride, a.n = n_vocab;
     a.temperature = temperature, a.top_k = top_k, a.top_p = top_p, a.min_p = min_p;
     a.u = u, a.out = out_idx;
-    a.chunks = (n_vocab + kBlock - 1) / kBlock;
+    a.chunks = chunks_of(n_vocab);
     a.ws = static_cast<uint8_t*>(ws);
     a.row_bytes = row_bytes_of(a.chunks);
-    TF_CHECK_ARG((long long)n_rows * a.chunks <= (long long)(UINT32_MAX / kRowThreads));
     const unsigned grid = (unsigned)n_rows * (unsigned)a.chunks;
     hipLaunchKernelGGL(tf_sample_stats_kernel, dim3(grid), dim3(kChunkThreads), 0,
                        tf_stream(stream), a);

@@ -156,3 +156,15 @@ def test_models_without_an_8_bit_cache(lib, shape):
     assert lib.tf_model_create_kv8(*args) == 801  # hipErrorNotSupported
     assert lib.tf_model_create_kv8(None, *args[1:]) == INVALID
     assert not out.value and lib.tf_model_use_kv8(None) == INVALID
+
+
+@pytest.mark.parametrize("n_vocab,most", [(10, 4194303), (8192, 4194303), (8193, 2097151),
+                                          (151936, 220752), (524287, 65535)])
+def test_sample_rows(lib, n_vocab, most):
+    """Rows past a launch's 2^32 threads have no workspace, as tf_sample refuses them."""
+    f = lib.tf_sample_ws_bytes
+    assert f(most, n_vocab) == most * f(1, n_vocab) > 0
+    assert f(most + 1, n_vocab) == -1 and f(2**31 - 1, n_vocab) == -1
+    big = {**SAMPLE, "n_rows": most + 1, "n_vocab": n_vocab, "row_stride": n_vocab,
+           "ws_bytes": 2**62}
+    assert lib.tf_sample(*big.values(), None) == INVALID
