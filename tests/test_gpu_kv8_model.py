@@ -254,3 +254,40 @@ def test_a_cache_that_does_not_fit(gpu, kv8):
         DecodeModel(dict(cfg, max_seq=2**31 - 1), layers, emb, kv8=kv8)
     assert np.array_equal(gm.generate([1, 2], 3, use_graph=False), want)
     gm.close()
+
+
+@pytest.mark.parametrize("start", [1, 31, 257, 600])
+def test_steps_after_a_prompt_over_several_splits(gpu, start, monkeypatch):
+    """Steps over rows that a prompt stored, in a cache that the attention splits (16 parts
+    of 704 rows), eager, and captured bit for bit.  Rows are held as step() holds them; the
+    logits by their norm, as a quotient that lies on a half may round either way in the Q8 of
+    an activation: in the head's (512 values, none above 8 of their RMS) it moves the logits
+    by 8 / 127 of that RMS times a column of the head, 8 / 127 / sqrt(512) = 2.8e-3 of their
+    norm.  Four of them are allowed for: 1.2e-2."""
+    cfg, layers, emb, make = build(1, 60, 704)
+    gm, rm = make(), Kv8Ref(cfg, layers, emb, 704)
+    gm.use_kv8()
+    rm.model = gm
+    assert gm.lib.tf_flash_decode_kv8_n_split(cfg["n_kv"], cfg["head_dim"], 704) == 16
+
+    def turned(x, w, eps, at, theta):  # the reference's angle, as steps have it
+        assert w is None and len(at) == 1
+        y = oracle.rope_neox(np.asarray(x).reshape(-1), x.shape[1], x.shape[2], int(at[0]), theta)
+        return y.reshape(x.shape), None
+
+    monkeypatch.setattr(ref, "norm_rope", turned)
+    toks = np.random.default_rng(start).integers(0, cfg["n_vocab"], start + 3).tolist()
+    gm.prefill(toks[:start], 0)
+    for li in range(cfg["n_layer"]):
+        k8, kd, v8, vd = gm.kv8_cache(li, start)
+        rm.rows[li][0][:start], rm.rows[li][1][:start] = ref.q8_values(k8, kd), ref.q8_values(v8, vd)
+    for pos in range(start, start + 3):
+        gm.forward(toks[pos], pos)
+        got, want = gm.logits().astype(np.float64), rm.step(toks[pos], pos).astype(np.float64)
+        assert np.linalg.norm(got - want) <= 1.2e-2 * np.linalg.norm(want), pos
+    last = gm.logits()
+    for graph in (False, True, True):
+        gm.prefill(toks[:start], 0)
+        nxt = gm.generate(toks[start:], 1, pos0=start, use_graph=graph)
+        assert np.array_equal(gm.logits(), last) and nxt[0] == int(np.argmax(last))
+    gm.close()
