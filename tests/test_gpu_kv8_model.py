@@ -291,3 +291,51 @@ def test_steps_after_a_prompt_over_several_splits(gpu, start, monkeypatch):
         nxt = gm.generate(toks[start:], 1, pos0=start, use_graph=graph)
         assert np.array_equal(gm.logits(), last) and nxt[0] == int(np.argmax(last))
     gm.close()
+
+
+@pytest.mark.parametrize("max_seq", [40, 700])
+def test_steps_of_a_q5_0_model(gpu, monkeypatch, max_seq):
+    """Layers whose norm, q, k and v (and over an f16 cache wo) are fused launches of their
+    own.  Attention in 64 bits over the rows that the model wrote; logits as
+    test_gpu_q05_model has them."""
+    from _model_ref import RefModelMixed
+    from _util import q8_0_dequant
+    from taraference_amd.model import DecodeModel
+    from test_gpu_q05_model import CFG as cfg
+    rng = np.random.default_rng(71)
+    layers = [synth.qwen05_layer(rng, cfg, li) for li in range(cfg["n_layer"])]
+    emb = synth.qwen05_embedding(rng, cfg)
+    gm = DecodeModel(dict(cfg, max_seq=max_seq), layers, emb, kv8=True)
+    rm = RefModelMixed(cfg, layers, emb, 16)
+
+    def attend(q, K, V, h, kv, hd, pos, split, scale):
+        li = next(i for i, k in enumerate(rm.K) if k is K)
+        k8, kd, v8, vd = gm.kv8_cache(li, pos + 1)
+        return ref.attention(np.asarray(q).reshape(h, hd), ref.q8_values(k8, kd),
+                             ref.q8_values(v8, vd), kv, scale)[0].astype(np.float32).reshape(-1)
+
+    monkeypatch.setattr(oracle, "flash_partial", attend)
+    monkeypatch.setattr(oracle, "flash_reduce", lambda out, h, hd, split: out)
+    nb = cfg["n_embd"] // 32
+    wmax = float(np.abs(q8_0_dequant(emb[0][:, : nb * 34].reshape(-1, 34))).max())
+    toks = rng.integers(0, cfg["n_vocab"], 12).tolist()
+    for pos, tok in enumerate(toks):
+        gm.forward(tok, pos)
+        got, want = gm.logits().astype(np.float64), rm.step(tok, pos)[0].astype(np.float64)
+        _, d8 = oracle.quantize_q8(rm.head_x)
+        tol = 2e-3 * np.sqrt(np.mean(want**2)) + 4 * float(d8.max()) * wmax
+        assert np.abs(got - want).max() <= tol, pos
+        k8, kd, v8, vd = (a[pos:] for a in gm.kv8_cache(0, pos + 1))
+        for q, d, bits in ((k8, kd, rm.K[0][pos]), (v8, vd, rm.V[0][pos])):
+            r = bits.view(np.float16).astype(np.float64)
+            step = np.repeat(d.astype(np.float64), 32, axis=1)[0]
+            near = 2.0**-11 * np.abs(r) + 2.1e-4 * np.sqrt(np.mean(r * r))
+            assert (np.abs(ref.q8_values(q, d)[0] - r) <= (0.5 + 2.0**-15) * step + near).all(), pos
+    last = gm.logits()
+    for graph in (False, True, True):
+        gm.generate(toks, 1, use_graph=graph)
+        assert np.array_equal(gm.logits(), last)
+    u = np.linspace(0.05, 0.95, 6).astype(np.float32)
+    eager = gm.generate_sampled(toks[:3], u, temperature=0.8, top_k=9, use_graph=False)
+    assert np.array_equal(gm.generate_sampled(toks[:3], u, temperature=0.8, top_k=9), eager)
+    gm.close()
