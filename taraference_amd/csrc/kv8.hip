@@ -18,7 +18,7 @@
 // so a lane moves 16 of the wider side at once; VEC false: a value a lane, for rows
 // that are not so aligned.  32768 f16 rows of 512, K and V (67 MB in, 38 out): 21.8 us,
 // 4.8 TB/s, with the VALU busy for 11 of them;
-// read back as f32 (38 in, 134 out) 25.3 us, 6.8 TB/s with what the last-level cache holds.
+// read back as f32 (38 in, 134 out) 25.2 us, 6.8 TB/s with what the last-level cache holds.
 typedef _Float16 tf_h2x __attribute__((ext_vector_type(2)));
 
 struct TfKv8Rows {
@@ -137,10 +137,10 @@ __global__ __launch_bounds__(256) void tf_kv8_read_kernel(const int8_t* __restri
 // % 16, g = l / 16: A[n][8g ..], B[8g ..][n], C[4g + r][n]):
 //   K Q^T  one k step is one scale group: A = 8 bytes of token n (or 16 + n), as
 //          f16 (exact), B = 8 dims of head n in two f16 parts after a power of
-//          two of the head's own (2^-22 of its largest); the sums of a group are f32 and take the
-//          token's scale there.
+//          two of the head's own (2^-22 of its largest); the sums of a group are f32
+//          and take the token's scale there.
 //   softmax of head n over the lane's tokens 4g + r and 16 + 4g + r, in f32.
-//          The maximum and the exponent below are renewed, and O rescaled, only
+//          The maximum and the factor f below are renewed, and O rescaled, only
 //          where a lane found a larger one.
 //   V^T P^T with the tokens in the order in which the lane has them: A = 8 tokens
 //          of dim n (ds_read_b64_tr_b8), as f16 (exact); B = p vd[t][g] f, for each
@@ -148,10 +148,10 @@ __global__ __launch_bounds__(256) void tf_kv8_read_kernel(const int8_t* __restri
 //          keeps every p vd f below 2^15 and the largest met so far (in the weights of
 //          the maximum so far) within 2^12 of that, so the parts end at 2^-28 of the
 //          largest product or below, whatever the scales of rows without weight.
-// 131072 tokens of 28/4 heads of 128 (151 MB): 36 us and 4.7 for the merge, 4.2 TB/s of
+// 131072 tokens of 28/4 heads of 128 (151 MB): 35.8 us and 4.7 for the merge, 4.2 TB/s of
 // the 5.8 that a plain read reaches; the copies alone take 30, and conversions, splits
-// and exponentials keep the VALU busy for 17 beside them.  5001 tokens of
-// 14/2 heads of 64: 5.4 + 3.7 us; 512 of 16/2 of 128: 6.8 + 2.8; there a launch's chain
+// and exponentials keep the VALU busy for 18 beside them.  5001 tokens of
+// 14/2 heads of 64: 5.5 + 3.7 us; 512 of 16/2 of 128: 6.9 + 2.7; there a launch's chain
 // of query, first tile and merge is what there is.
 //
 // LDS rows keep their 16-byte chunks xor-ed with the row (the copies' sources

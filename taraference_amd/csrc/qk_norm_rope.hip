@@ -51,8 +51,9 @@ __device__ __forceinline__ float turns(long long pos, int i, int head_dim, doubl
 // a thread a pair, into LDS.  One token a workgroup (of few tokens, `share` heads of
 // one), four where they fill the CUs.
 // Bound by its bytes: 4096 tokens of 28 + 8 heads of 128 into the 8-bit cache move 139
-// MB in 30.4 us (4.6 TB/s); 777 tokens of 16 + 2 heads of 128 to f32 rows 8.9 us, one
-// token of 14 + 2 heads of 64 4.0, which is a launch's chain of loads.
+// MB in 31.2 us (4.5 TB/s); 777 tokens of 16 + 2 heads of 128 to f32 rows 8.8 us (heads in
+// passes of 16 a token, so the second has 2); one token of 14 + 2 heads of 64 3.8, where a
+// row that is stored without angles takes 1.7: f64 exponentials, sines and a barrier.
 // F32: the angle as tf_rope_neox and the prompts' kernels form it.
 template <int HD, Dest D, int TOK, bool F32 = false>
 __global__ __launch_bounds__(256) void tf_qk_norm_rope_vec_kernel(QkArgs a, int n_tok, int share) {

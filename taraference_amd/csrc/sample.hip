@@ -33,11 +33,12 @@
 // among more elements than the list holds (equal logits by the thousand), whose logits
 // the bins cannot hold (an infinite one, T below 1e-37), or whose u is below 2^-20, is
 // selected by radix passes over the row itself in the third launch: the same cut, found by
-// one workgroup (151936 equal logits with top-p 312 us).  Bins of the row's own size keep
-// others from there: logits within 0.1 of each other, or T = 3, take the time of any row.
+// one workgroup (151936 equal logits with top-p 317 us, u = 0 with no filter 65).  Bins of
+// the row's own size keep others from there: logits within 0.1 of each other, or T = 3,
+// take the time of any row.
 //
-// One row of 151936 with all filters: 9 + 8 + 4.5 us, without filters 5.6 + 4.5; bound by
-// chains of loads and barriers (19 workgroups, then one).  64 rows with top-p: 23.2 + 19.9
+// One row of 151936 with all filters: 8 + 8 + 4.7 us, without filters 5.5 + 4.7; bound by
+// chains of loads and barriers (19 workgroups, then one).  64 rows with top-p: 23.2 + 20.0
 // + 14.7 us.  There the first launch has its VALU busy for 16 us (64 instructions for an
 // element's bin and weight); without exponentials it took 6.5 less, without the atomics 1.
 // 1216 workgroups run in two rounds of three a CU: more a CU would spill registers, and
@@ -58,7 +59,7 @@ constexpr int kMinFine = -240;      // and wider where their numbers would pass 
 constexpr float kNoWeight = 5560.f; // bins below the largest from which exp2_neg() gives 0
 constexpr float kPerZ = 8.f;
 constexpr int kList = 8192;         // elements of a row's list, and
-constexpr int kChunkList = 2048;    // of a chunk's part of it
+constexpr int kChunkList = 2048;    // of a chunk's part of it, three quarters of its workspace
 constexpr int kChunkThreads = 512, kChunkWaves = kChunkThreads / 64;
 constexpr int kBlock = 16 * kChunkThreads;  // elements of a chunk: its workgroup's registers
 constexpr int kMaxVocab = 1 << 19;
