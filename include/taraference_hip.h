@@ -644,7 +644,7 @@ int tf_model_generate_sampled(tf_model *m, const int *forced, int n_forced,
 /* No counterpart in the reference: hold the K/V cache in 8 bits (see
  * tf_kv8_write) from here on, n_layer * max_seq * n_kv * head_dim * 2.25 bytes
  * in place of 4; until this returns there is room for both.  Rows written before
- * are lost.  Steps take path 0 with their rows stored in 8 bits, turned by
+ * are lost, and steps that the caller captured must not be replayed.  Steps take path 0 with their rows stored in 8 bits, turned by
  * tf_rope_neox's angle as prompts' are, and tf_flash_decode_kv8 in it; prompts
  * attend over the rows read back in f16 (room for one layer's, taken on the first
  * prompt), and over their own as f16 has them, from which they are stored.
